@@ -362,6 +362,40 @@ def ce_backward(logits2, target, logz, grad_loss, grad_z, vocab_start: int):
     return ref.ce_backward(logits2, target, logz, grad_loss, grad_z, vocab_start)
 
 
+# ============================================================================ cross entropy of a linear head (no logits)
+def linear_ce_forward(x2: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, vocab_start: int, finish: bool):
+    """Softmax statistics of the scores ``x2 @ weight.T`` ([T, H], [V, H]), which are never materialised.  ``finish`` (``weight`` is the
+    whole vocabulary): (logZ, loss) per token; otherwise the shard's (max, sum exp, target score or 0) like ``ce_partials``."""
+    if _use_native(x2):
+        from nanotron_b200.ops import native_ce
+
+        native_ce.check_operands(x2, weight, target)
+        return native_ce.forward(x2, weight, target, vocab_start, finish)
+    m, s, t = ref.linear_ce_partials(x2, weight, target, vocab_start)
+    if not finish:
+        return m, s, t
+    logz = m + torch.log(s)
+    return logz, logz - t
+
+
+def linear_ce_backward(x2, weight, target, logz, grad_loss, grad_z, vocab_start: int, need_dx: bool = True, need_dw: bool = True):
+    """(dx, dw) of the losses.  A weight that carries an fp32 ``main_grad`` gets its gradient added there, and None is returned for it."""
+    main_grad = getattr(weight, "main_grad", None) if need_dw else None
+    if _use_native(x2):
+        from nanotron_b200.ops import native_ce
+
+        direct = main_grad is not None and main_grad.dtype == torch.float32 and main_grad.stride(1) == 1 and main_grad.stride(0) % 8 == 0 and main_grad.data_ptr() % 16 == 0
+        dx, dw = native_ce.backward(x2, weight, target, logz, grad_loss, grad_z, vocab_start, need_dx, need_dw, main_grad if direct else None)
+        if direct:
+            return dx, None
+    else:
+        dx, dw = ref.linear_ce_backward(x2, weight, target, logz, grad_loss, grad_z, vocab_start)
+    if main_grad is not None:
+        main_grad.add_(dw)
+        dw = None
+    return (dx if need_dx else None), (dw if need_dw else None)
+
+
 # ============================================================================ attention
 class _FlashAttnVarlen(torch.autograd.Function):
     @staticmethod

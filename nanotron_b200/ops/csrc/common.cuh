@@ -16,12 +16,17 @@
 // device's primary context to a thread at its first runtime call that needs one; a fresh thread whose first CUDA work is one
 // of the tensor-map builders below has none yet (seen with autograd worker threads on device 0, where the framework skips
 // cudaSetDevice because device 0 is already the thread's default): the encode call then fails and the entry point would
-// report the arguments as unsupported.  Binding once per thread costs two runtime calls.
+// report the arguments as unsupported.  Binding once per thread costs a few runtime calls.  cudaFree(nullptr) counts as an unsafe
+// call while a stream is being captured (a thread whose first product is inside a captured backward pass would end the capture), so
+// the thread's capture mode is relaxed around it.
 static inline void ntb_bind_context_to_thread() {
   static thread_local bool bound = false;
   if (bound) return;
   int dev = 0;
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  const bool relaxed = cudaThreadExchangeStreamCaptureMode(&mode) == cudaSuccess;
   if (cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess && cudaFree(nullptr) == cudaSuccess) bound = true;
+  if (relaxed) cudaThreadExchangeStreamCaptureMode(&mode);
 }
 
 static inline int ntb_check_launch() {

@@ -1,0 +1,287 @@
+// Cross entropy of a linear head without its logits (sm_100a).
+//
+//   l[t,v] = sum_h x[t,h] w[v,h]      logZ[t] = log sum_v exp l[t,v]      loss[t] = logZ[t] - l[t, y_t]
+//   d[t,v] = coef[t] exp(l[t,v] - logZ[t]) - g[t] [v == y_t]             dx = d w        dw = d^T x
+//
+// Forward: one GEMM over the whole vocabulary on CTA pairs (gemm2_core.cuh) whose epilogue keeps, per token and 256-column tile, only
+// (largest score, sum of exponentials); a small kernel joins the tiles of a token.  Scores never leave the tensor memory, and they
+// are used in fp32 (logits written in bf16 are off by up to 2^-9 of their value, several percent of a probability).
+// Backward: the vocabulary is cut into pieces; for each piece the scores are computed again, the epilogue turns them into d (bf16,
+// one rounding), and two plain products take d to dx (summed over the pieces in fp32) and to the piece's rows of dw.  Only one
+// piece of d is alive.  d is kept in units of the largest |g| (`ce_row_coefficients`) and the products are scaled back by that one
+// number in fp32: with a masked mean every g is the same number, and rounding -g (1 - p) to bf16 would shift the dominant entry of
+// every row by the same relative amount (up to 2^-8), an error that no summation averages out; in units of g it is -(1 - p).
+#include "gemm2_core.cuh"
+
+namespace {
+
+constexpr int CE_JOIN_ROWS = 32;
+constexpr int CE_JOIN_PARTS = 16;
+
+// One block per 32 tokens; 16 groups of threads share the tiles of a token.  Reads of `part` are contiguous over the tokens.
+__global__ void __launch_bounds__(CE_JOIN_ROWS * CE_JOIN_PARTS)
+ce_join_kernel(const float2* __restrict__ part, const float* __restrict__ tgt, const int64_t* __restrict__ target, int64_t vocab_start, int vocab, int tiles,
+               int rows, float* __restrict__ out_max, float* __restrict__ out_sum, float* __restrict__ out_tgt, float* __restrict__ logz,
+               float* __restrict__ loss) {
+  __shared__ float sm[CE_JOIN_PARTS][CE_JOIN_ROWS], ss[CE_JOIN_PARTS][CE_JOIN_ROWS];
+  const int lane = threadIdx.x & 31, grp = threadIdx.x >> 5;
+  const int row = blockIdx.x * CE_JOIN_ROWS + lane;
+  float m = -INFINITY, s = 0.f;
+  if (row < rows) {
+    for (int i = grp; i < tiles; i += CE_JOIN_PARTS) {
+      const float2 p = part[static_cast<int64_t>(i) * rows + row];
+      const float nm = fmaxf(m, p.x);
+      const float base = nm == -INFINITY ? 0.f : nm * P_LOG2E;
+      s = s * p_ex2(fmaf(m, P_LOG2E, -base)) + p.y * p_ex2(fmaf(p.x, P_LOG2E, -base));
+      m = nm;
+    }
+  }
+  sm[grp][lane] = m;
+  ss[grp][lane] = s;
+  __syncthreads();
+  if (grp != 0 || row >= rows) return;
+  float gm = -INFINITY, gs = 0.f;
+#pragma unroll
+  for (int i = 0; i < CE_JOIN_PARTS; i++) gm = fmaxf(gm, sm[i][lane]);
+  const float base = gm == -INFINITY ? 0.f : gm * P_LOG2E;
+#pragma unroll
+  for (int i = 0; i < CE_JOIN_PARTS; i++) gs += ss[i][lane] * p_ex2(fmaf(sm[i][lane], P_LOG2E, -base));
+  const int64_t rel = target[row] - vocab_start;
+  const float t = (rel >= 0 && rel < vocab) ? tgt[row] : 0.f;
+  if (out_max != nullptr) {
+    out_max[row] = gm;
+    out_sum[row] = gs;
+    out_tgt[row] = t;
+  }
+  if (logz != nullptr) {
+    const float lz = gm + logf(gs);
+    logz[row] = lz;
+    loss[row] = lz - t;
+  }
+}
+
+// coef = (g + gz) / unit, g = g / unit with unit = the largest |g| or |g + gz| (1 where that is no use as a divisor).  One block.
+__global__ void __launch_bounds__(1024) ce_row_coefficients_kernel(const float* __restrict__ g, const float* __restrict__ gz, int rows, float* __restrict__ coef,
+                                                                    float* __restrict__ gn, float* __restrict__ unit) {
+  __shared__ float scratch[32];
+  float m = 0.f;
+  for (int i = threadIdx.x; i < rows; i += blockDim.x) m = fmaxf(m, fmaxf(fabsf(g[i]), gz ? fabsf(g[i] + gz[i]) : 0.f));
+  m = block_max(m, scratch);
+  const float u = (m > 1e-30f && m < 1e30f) ? m : 1.f;
+  if (threadIdx.x == 0) *unit = u;
+  for (int i = threadIdx.x; i < rows; i += blockDim.x) {
+    coef[i] = (gz ? g[i] + gz[i] : g[i]) / u;
+    gn[i] = g[i] / u;
+  }
+}
+
+// out = bf16(*unit * acc), eight elements a thread.
+__global__ void __launch_bounds__(256) ce_scale_cast_kernel(const float* __restrict__ acc, const float* __restrict__ unit, __nv_bfloat16* __restrict__ out, int64_t n8) {
+  const float u = *unit;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < n8; i += static_cast<int64_t>(gridDim.x) * 256) {
+    Vec8<float> a;
+    float f[8];
+    a.load(acc + i * 8);
+    a.to_float(f);
+#pragma unroll
+    for (int j = 0; j < 8; j++) f[j] *= u;
+    Vec8<__nv_bfloat16> o;
+    o.from_float(f);
+    o.store(out + i * 8);
+  }
+}
+
+template <class K>
+int ce_configure(K kern, bool (&done)[64]) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return NTB_ERR_LAUNCH;
+  if (!done[dev]) {
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, P_SMEM) != cudaSuccess) {
+      cudaGetLastError();
+      return NTB_ERR_LAUNCH;
+    }
+    done[dev] = true;
+  }
+  return NTB_OK;
+}
+
+int ce_band(int M, int K) {
+  const int tiles_m = (M + 2 * P_BLOCK_M - 1) / (2 * P_BLOCK_M);
+  int band = static_cast<int>(40000000ll / (512ll * K));  // rows of A that stay in L2 while B streams: about 40 MB
+  if (band < 2) band = 2;
+  return band > tiles_m ? tiles_m : band;
+}
+
+template <bool A_MN, bool B_MN, int OUT, class EXT>
+int ce_launch(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& td, int M, int N, int K, const PSched& sched, const CUtensorMap& tws, const EXT& ext,
+              int* status, int num_sms, cudaStream_t stream) {
+  auto kern = gemm2_tcgen05_kernel<A_MN, B_MN, OUT, P_MAX_STAGES, EXT>;
+  static bool done[64] = {};
+  if (int rc = ce_configure(kern, done)) return rc;
+  static const PPeerMaps no_maps = {};
+  int pairs = num_sms / 2;
+  if (sched.total_units < pairs) pairs = sched.total_units;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(2 * pairs), 1, 1);
+  cfg.blockDim = dim3(P_THREADS, 1, 1);
+  cfg.dynamicSmemBytes = P_SMEM;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, kern, ta, tb, td, M, N, K, ce_band(M, K), status, PFuse(), no_maps, sched, tws, ta, ext) != cudaSuccess) {
+    cudaGetLastError();
+    return NTB_ERR_LAUNCH;
+  }
+  return ntb_check_launch();
+}
+
+PSched ce_whole_tiles(int M, int N, int K, bool& fits) {
+  const long long tiles = static_cast<long long>((M + 2 * P_BLOCK_M - 1) / (2 * P_BLOCK_M)) * ((N + P_BLOCK_N - 1) / P_BLOCK_N);
+  fits = tiles < (1ll << 30);
+  PSched sc;
+  sc.total_units = sc.full_units = static_cast<int>(tiles);
+  sc.split = 1;
+  sc.kb_per = (K + P_BLOCK_K - 1) / P_BLOCK_K;
+  return sc;
+}
+
+bool ce_operand_ok(const void* p, int64_t ld) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld % 64 == 0; }
+
+}  // namespace
+
+// part: fp32 pairs [ceil(V / 256)][T]; tgt: fp32 [T] (written where the target is in [vocab_start, vocab_start + V)).
+// x [T, H] and w [V, H] bf16, rows 16-byte aligned at pitches ldx, ldw (multiples of 64), H a multiple of 64.
+NTB_EXPORT int ntb_linear_ce_stats(const void* x, int64_t ldx, const void* w, int64_t ldw, const int64_t* target, int64_t vocab_start, int T, int V, int H, void* part,
+                                   float* tgt, int* status, int num_sms, cudaStream_t stream) {
+  if (T <= 0 || V <= 0 || H <= 0 || H % 64 || !ce_operand_ok(x, ldx) || !ce_operand_ok(w, ldw) || num_sms < 2 || !p_get_encode()) return NTB_ERR_ARG;
+  bool fits;
+  const PSched sched = ce_whole_tiles(T, V, H, fits);
+  CUtensorMap ta, tb;
+  if (!fits || !p_map_kmajor(&ta, x, T, H, ldx) || !p_map_kmajor(&tb, w, V, H, ldw)) return NTB_ERR_ARG;
+  PCeArgs a;
+  a.target = target;
+  a.col0 = vocab_start;
+  a.part = static_cast<float2*>(part);
+  a.tgt = tgt;
+  return ce_launch<false, false, P_OUT_CE_STATS>(ta, tb, ta, T, V, H, sched, ta, a, status, num_sms, stream);
+}
+
+// Joins the tiles of every token.  out_max / out_sum / out_tgt (all or none): the three numbers that vocabulary shards exchange;
+// logz / loss (both or none): the finished values where this is the whole vocabulary.
+NTB_EXPORT int ntb_linear_ce_join(const void* part, const float* tgt, const int64_t* target, int64_t vocab_start, int T, int V, float* out_max, float* out_sum,
+                                  float* out_tgt, float* logz, float* loss, cudaStream_t stream) {
+  if (T <= 0 || V <= 0 || (out_max != nullptr) != (out_sum != nullptr) || (out_max != nullptr) != (out_tgt != nullptr) || (logz != nullptr) != (loss != nullptr)) return NTB_ERR_ARG;
+  const int tiles = (V + P_BLOCK_N - 1) / P_BLOCK_N;
+  ce_join_kernel<<<(T + CE_JOIN_ROWS - 1) / CE_JOIN_ROWS, CE_JOIN_ROWS * CE_JOIN_PARTS, 0, stream>>>(static_cast<const float2*>(part), tgt, target, vocab_start, V, tiles, T, out_max,
+                                                                                                     out_sum, out_tgt, logz, loss);
+  return ntb_check_launch();
+}
+
+// g, gz (or null), coef, gn: fp32 [T]; unit: one fp32.
+NTB_EXPORT int ntb_linear_ce_row_coefficients(const float* g, const float* gz, int T, float* coef, float* gn, float* unit, cudaStream_t stream) {
+  if (T <= 0) return NTB_ERR_ARG;
+  ce_row_coefficients_kernel<<<1, 1024, 0, stream>>>(g, gz, T, coef, gn, unit);
+  return ntb_check_launch();
+}
+
+// d [T, V] bf16 at pitch ldd (a multiple of 64, at least V rounded up to 64; the columns up to there are written, as zeros), for the V
+// rows of w from vocabulary entry `vocab_start` on.
+NTB_EXPORT int ntb_linear_ce_dlogits(const void* x, int64_t ldx, const void* w, int64_t ldw, const int64_t* target, int64_t vocab_start, const float* logz,
+                                     const float* coef, const float* gn, int T, int V, int H, void* d, int64_t ldd, int* status, int num_sms, cudaStream_t stream) {
+  if (T <= 0 || V <= 0 || H <= 0 || H % 64 || !ce_operand_ok(x, ldx) || !ce_operand_ok(w, ldw) || !ce_operand_ok(d, ldd) || num_sms < 2 || !p_get_encode()) return NTB_ERR_ARG;
+  const int64_t width = (static_cast<int64_t>(V) + 63) / 64 * 64;
+  if (ldd < width) return NTB_ERR_ARG;
+  bool fits;
+  const PSched sched = ce_whole_tiles(T, V, H, fits);
+  CUtensorMap ta, tb, td;
+  if (!fits || !p_map_kmajor(&ta, x, T, H, ldx) || !p_map_kmajor(&tb, w, V, H, ldw) || !p_map_out(&td, d, T, width, ldd, false)) return NTB_ERR_ARG;
+  PCeArgs a;
+  a.target = target;
+  a.col0 = vocab_start;
+  a.logz = logz;
+  a.coef = coef;
+  a.g = gn;
+  return ce_launch<false, false, P_OUT_CE_GRAD>(ta, tb, td, T, V, H, sched, ta, a, status, num_sms, stream);
+}
+
+// How the dx product [T, H] over V is cut along V: with fewer tiles than CTA pairs (few tokens) every tile becomes `split` chunks
+// whose fp32 partial sums go through a workspace and are added in chunk order.  Returns the chunks per tile (1: not cut).
+NTB_EXPORT int ntb_linear_ce_dx_split(int T, int V, int H, int num_sms) {
+  const int pairs = num_sms / 2;
+  const int tiles = ((T + 255) / 256) * ((H + 255) / 256);
+  const int kb = (V + P_BLOCK_K - 1) / P_BLOCK_K;
+  if (tiles >= 2 * pairs) return 1;
+  // fewest rounds of (chunk length + a fixed share for the start and the hand-over of a chunk, about eight k-blocks)
+  int best = 1;
+  long long best_cost = -1;
+  for (int s = 1; s <= 64 && s * 8 <= kb + 7 && tiles * s <= 4 * pairs; s++) {
+    const long long rounds = (static_cast<long long>(tiles) * s + pairs - 1) / pairs;
+    const long long cost = rounds * ((kb + s - 1) / s + 8);
+    if (best_cost < 0 || cost < best_cost) best = s, best_cost = cost;
+  }
+  return best;
+}
+
+// dx (+)= d w over the V columns of d.  mode 0: dx bf16 = unit * sum; 1: dx fp32 = sum; 2: dx fp32 += sum (one launch at a time on a
+// buffer).  ws: fp32, split * tiles * 65536 elements when split > 1 (not needed otherwise).
+NTB_EXPORT int ntb_linear_ce_dx(const void* d, int64_t ldd, const void* w, int64_t ldw, void* dx, int64_t lddx, int T, int V, int H, int mode, const float* unit,
+                                int split, float* ws, int* status, int num_sms, cudaStream_t stream) {
+  if (T <= 0 || V <= 0 || H <= 0 || H % 64 || !ce_operand_ok(d, ldd) || !ce_operand_ok(w, ldw) || !ce_operand_ok(dx, lddx) || mode < 0 || mode > 2 || num_sms < 2 ||
+      split < 1 || (split > 1 && ws == nullptr) || (reinterpret_cast<uintptr_t>(ws) & 127) || !p_get_encode())
+    return NTB_ERR_ARG;
+  bool fits;
+  PSched sched = ce_whole_tiles(T, H, V, fits);
+  const int tiles = sched.total_units, kb = sched.kb_per;
+  CUtensorMap ta, tb, td;
+  if (!fits || !p_map_kmajor(&ta, d, T, V, ldd) || !p_map_mnmajor(&tb, w, H, V, ldw) || !p_map_out(&td, dx, T, H, lddx, mode != 0)) return NTB_ERR_ARG;
+  CUtensorMap tws = td;
+  if (split > 1) {
+    sched.full_units = 0;
+    sched.split = split;
+    sched.kb_per = (kb + split - 1) / split;
+    sched.total_units = tiles * split;
+    if (!p_map_out(&tws, ws, static_cast<int64_t>(tiles) * split * 2 * P_BLOCK_M, P_BLOCK_N, P_BLOCK_N, true)) return NTB_ERR_ARG;
+  }
+  PAlpha a;
+  a.alpha = mode == 0 ? unit : nullptr;
+  int rc;
+  if (mode == 0) rc = ce_launch<false, true, P_OUT_BF16>(ta, tb, td, T, H, V, sched, tws, a, status, num_sms, stream);
+  else if (mode == 1) rc = ce_launch<false, true, P_OUT_F32>(ta, tb, td, T, H, V, sched, tws, a, status, num_sms, stream);
+  else rc = ce_launch<false, true, P_OUT_F32_ACCUM>(ta, tb, td, T, H, V, sched, tws, a, status, num_sms, stream);
+  if (rc != NTB_OK || split == 1) return rc;
+  const int tiles_m = (T + 2 * P_BLOCK_M - 1) / (2 * P_BLOCK_M), tiles_n = (H + P_BLOCK_N - 1) / P_BLOCK_N, band = ce_band(T, V);
+  if (mode == 0) gemm2_split_fixup_kernel<P_OUT_BF16><<<tiles * 8, 256, 0, stream>>>(ws, dx, lddx, T, H, kb, sched, tiles_m, tiles_n, band, 0, unit);
+  else if (mode == 1) gemm2_split_fixup_kernel<P_OUT_F32><<<tiles * 8, 256, 0, stream>>>(ws, dx, lddx, T, H, kb, sched, tiles_m, tiles_n, band, 0);
+  else gemm2_split_fixup_kernel<P_OUT_F32_ACCUM><<<tiles * 8, 256, 0, stream>>>(ws, dx, lddx, T, H, kb, sched, tiles_m, tiles_n, band, 0);
+  return ntb_check_launch();
+}
+
+// out [n] bf16 = unit * acc [n] fp32; n a multiple of 8, both 16-byte aligned.
+NTB_EXPORT int ntb_linear_ce_scale_cast(const float* acc, const float* unit, void* out, int64_t n, cudaStream_t stream) {
+  if (n <= 0 || n % 8 || ((reinterpret_cast<uintptr_t>(acc) | reinterpret_cast<uintptr_t>(out)) & 15)) return NTB_ERR_ARG;
+  int64_t blocks = (n / 8 + 255) / 256;
+  if (blocks > 148 * 8) blocks = 148 * 8;
+  ce_scale_cast_kernel<<<static_cast<unsigned>(blocks), 256, 0, stream>>>(acc, unit, static_cast<__nv_bfloat16*>(out), n / 8);
+  return ntb_check_launch();
+}
+
+// Rows of the weight gradient: dw [V, H] = unit * d^T x (accumulate 0: bf16 store; 1: added to fp32 dw).
+NTB_EXPORT int ntb_linear_ce_dw(const void* d, int64_t ldd, const void* x, int64_t ldx, void* dw, int64_t lddw, int T, int V, int H, int accumulate, const float* unit,
+                                int* status, int num_sms, cudaStream_t stream) {
+  if (T <= 0 || V <= 0 || H <= 0 || H % 64 || !ce_operand_ok(d, ldd) || !ce_operand_ok(x, ldx) || (reinterpret_cast<uintptr_t>(dw) & 15) || lddw % 8 || num_sms < 2 ||
+      !p_get_encode())
+    return NTB_ERR_ARG;
+  bool fits;
+  const PSched sched = ce_whole_tiles(V, H, T, fits);
+  CUtensorMap ta, tb, td;
+  if (!fits || !p_map_mnmajor(&ta, d, V, T, ldd) || !p_map_mnmajor(&tb, x, H, T, ldx) || !p_map_out(&td, dw, V, H, lddw, accumulate != 0)) return NTB_ERR_ARG;
+  PAlpha a;
+  a.alpha = unit;
+  if (accumulate) return ce_launch<true, true, P_OUT_F32_ACCUM>(ta, tb, td, V, H, T, sched, ta, a, status, num_sms, stream);
+  return ce_launch<true, true, P_OUT_BF16>(ta, tb, td, V, H, T, sched, ta, a, status, num_sms, stream);
+}

@@ -86,10 +86,11 @@ def _declare(L):
         L.ntb_dp_adamw_allgather.argtypes = [c_void_p] * 5 + [c_int, c_int, c_int64, c_int64] + [c_void_p] * 3 + [c_int] + [c_float] * 5 + [c_void_p, c_void_p]
     for fn in ("ntb_norm_fwd", "ntb_norm_bwd", "ntb_rope", "ntb_swiglu_fwd", "ntb_swiglu_bwd", "ntb_ce_partials", "ntb_ce_backward", "ntb_adamw_flat", "ntb_sumsq"):
         getattr(L, fn).restype = c_int
-    from nanotron_b200.ops import native_gemm, native_attn  # noqa: F401  (declare their symbols when present)
+    from nanotron_b200.ops import native_gemm, native_attn, native_ce  # noqa: F401  (declare their symbols when present)
 
     native_gemm.declare(L)
     native_attn.declare(L)
+    native_ce.declare(L)
 
 
 def _stream(t: torch.Tensor) -> int:

@@ -161,6 +161,42 @@ def ce_backward(logits, target, logz, grad_loss, grad_z, vocab_start: int):
     return g.to(logits.dtype)
 
 
+def _wide(t: torch.Tensor) -> torch.Tensor:
+    return t if t.dtype == torch.float64 else t.float()
+
+
+def linear_ce_partials(x, weight, target, vocab_start: int, piece: int = 8192):
+    """``ce_partials`` of ``x @ weight.T`` ([T, H] and [V, H]), computed ``piece`` vocabulary entries at a time: the scores of one piece
+    are all that exists of the logits."""
+    xf, V = _wide(x), weight.shape[0]
+    m = torch.full((x.shape[0],), float("-inf"), dtype=xf.dtype, device=x.device)
+    s, t = torch.zeros_like(m), torch.zeros_like(m)
+    for a in range(0, V, piece):
+        l = xf @ _wide(weight[a : a + piece]).t()
+        nm = torch.maximum(m, l.max(dim=-1).values)
+        s = s * torch.exp(m - nm) + torch.exp(l - nm.unsqueeze(-1)).sum(-1)
+        m = nm
+        local = target - vocab_start - a
+        inside = (local >= 0) & (local < l.shape[1])
+        t = torch.where(inside, l.gather(-1, local.clamp(0, l.shape[1] - 1).unsqueeze(-1)).squeeze(-1), t)
+    return m, s, t
+
+
+def linear_ce_backward(x, weight, target, logz, grad_loss, grad_z, vocab_start: int, piece: int = 8192):
+    """Gradients (of ``x`` and ``weight``, in their types) of the losses whose log-partition is ``logz``, by pieces of the vocabulary."""
+    xf = _wide(x)
+    dx, dw = torch.zeros_like(xf), torch.empty(weight.shape, dtype=xf.dtype, device=x.device)
+    for a in range(0, weight.shape[0], piece):
+        wp = _wide(weight[a : a + piece])
+        d = torch.exp(xf @ wp.t() - logz.unsqueeze(-1)) * (grad_loss if grad_z is None else grad_loss + grad_z).unsqueeze(-1)
+        local = target - vocab_start - a
+        sub = torch.where((local >= 0) & (local < wp.shape[0]), grad_loss, torch.zeros_like(grad_loss))
+        d.scatter_add_(-1, local.clamp(0, wp.shape[0] - 1).unsqueeze(-1), -sub.unsqueeze(-1).to(d.dtype))
+        dx += d @ wp
+        dw[a : a + piece] = d.t() @ xf
+    return dx.to(x.dtype), dw.to(weight.dtype)
+
+
 # ------------------------------------------------------------------ attention
 def attention_varlen(q, k, v, cu_seqlens_q, cu_seqlens_k, causal: bool = True, softmax_scale: Optional[float] = None, window: Optional[int] = None, return_lse: bool = False, q_offsets=None):
     """q: [Tq, Hq, D], k/v: [Tk, Hkv, D]; sequences delimited by cu_seqlens (int32 [B+1]).

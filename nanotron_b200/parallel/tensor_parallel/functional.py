@@ -21,6 +21,7 @@ from __future__ import annotations
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd.function import once_differentiable
 
 import nanotron_b200.distributed as dist
 from nanotron_b200 import ops
@@ -280,9 +281,90 @@ def sharded_cross_entropy_with_z_loss(sharded_logits, target, group, dtype=None,
     return _ShardedCrossEntropy.apply(sharded_logits, target, group, float(z_loss_coef))
 
 
+# ----------------------------------------------------------------------------- cross entropy of a vocabulary-sharded linear head
+class _LinearCrossEntropy(torch.autograd.Function):
+    """The head product and ``_ShardedCrossEntropy`` in one: the scores exist only on chip (forward) or one piece of the vocabulary at
+    a time (backward, which computes them again), so no tensor of tokens x vocabulary is kept between the two.  Saved for backward:
+    the hidden states, the weight and one log-partition per token."""
+
+    @staticmethod
+    def forward(ctx, x, weight, target, group, z_loss_coef: float):
+        tp = group.size() if group is not None else 1
+        rank = dist.get_rank(group) if tp > 1 else 0
+        lead = x.shape[:-1]
+        x2, tgt = x.reshape(-1, x.shape[-1]), target.reshape(-1).to(torch.int64).contiguous()
+        vocab_start = rank * weight.shape[0]
+        if x2.shape[0] == 0:
+            logz = loss = torch.zeros(0, dtype=torch.float32, device=x.device)
+        elif tp == 1:
+            logz, loss = ops.linear_ce_forward(x2, weight, tgt, 0, finish=True)
+        else:
+            local_max, local_sumexp, local_tgt = ops.linear_ce_forward(x2, weight, tgt, vocab_start, finish=False)
+            fused = ops.tp_fused.get_context(group) if x.is_cuda and ops.tp_fused.ENABLED else None
+            if fused is not None:
+                logz, loss = fused.ce_combine(local_max, local_sumexp, local_tgt)  # tp reduction by peer loads inside the kernel
+            else:
+                gmax = local_max.clone()
+                dist.all_reduce(gmax, op=dist.ReduceOp.MAX, group=group)
+                packed = torch.stack([local_sumexp * torch.exp(local_max - gmax), local_tgt])
+                dist.all_reduce(packed, op=dist.ReduceOp.SUM, group=group)
+                logz = gmax + torch.log(packed[0])
+                loss = logz - packed[1]
+        ctx.save_for_backward(x2, weight, tgt, logz)
+        ctx.vocab_start, ctx.shape, ctx.z = vocab_start, x.shape, z_loss_coef
+        return loss.view(lead), ((z_loss_coef * logz.square()).view(lead) if z_loss_coef > 0 else None)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_loss, grad_z):
+        x2, weight, tgt, logz = ctx.saved_tensors
+        need_dx, need_dw = ctx.needs_input_grad[:2]
+        if x2.shape[0] == 0:
+            return (x2.new_zeros(ctx.shape) if need_dx else None), (torch.zeros_like(weight) if need_dw else None), None, None, None
+        wide = logz.dtype
+        g = grad_loss.reshape(-1).to(wide).contiguous()
+        gz = 2.0 * ctx.z * logz * grad_z.reshape(-1).to(wide) if ctx.z > 0 else None
+        dx, dw = ops.linear_ce_backward(x2, weight, tgt, logz, g, gz, ctx.vocab_start, need_dx, need_dw)
+        return (dx.view(ctx.shape) if need_dx else None), dw, None, None, None
+
+
+def _check_linear_cross_entropy(x, weight, target, group):
+    if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1]:
+        raise ValueError(f"hidden states [..., H] and weight [V, H] expected, got {tuple(x.shape)} and {tuple(weight.shape)}")
+    if x.dtype != weight.dtype or not x.is_floating_point():
+        raise ValueError(f"hidden states and weight must have the same floating type, got {x.dtype} and {weight.dtype}")
+    if weight.shape[0] == 0:
+        raise ValueError("the vocabulary is empty")
+    if target.shape != x.shape[:-1] or target.dtype not in (torch.int64, torch.int32):
+        raise ValueError(f"one int64 or int32 target per token expected: hidden states {tuple(x.shape)}, targets {tuple(target.shape)} of {target.dtype}")
+
+
+def linear_cross_entropy(x, weight, target, group: Optional[dist.ProcessGroup] = None):
+    """Per-token cross entropy (fp32) of the head ``x @ weight.T`` without materialising its logits: x [..., H], ``weight`` [V / tp, H]
+    this rank's rows of the head, target [...] class indices of the whole vocabulary.  Differentiable in ``x`` and ``weight``; over
+    several ranks the gradient of ``x`` is this rank's part of the sum over ``group`` (feed ``x`` through ``differentiable_identity`` or
+    ``differentiable_all_gather``, as ``column_linear`` does).  A weight with an fp32 ``main_grad`` receives its gradient there.
+
+    A target outside the vocabulary counts as a class of score 0 without gradient, as in ``sharded_cross_entropy``: multiply such
+    rows by a mask.  On CUDA: bf16, H a multiple of 64 (anything else raises ValueError); one level of differentiation."""
+    _check_linear_cross_entropy(x, weight, target, group)
+    loss, _ = _LinearCrossEntropy.apply(x, weight, target, group, 0.0)
+    return loss
+
+
+def linear_cross_entropy_with_z_loss(x, weight, target, group: Optional[dist.ProcessGroup] = None, z_loss_coef: float = 1e-4):
+    """``linear_cross_entropy`` and the per-token term ``z_loss_coef * logZ^2`` (None when the coefficient is 0)."""
+    _check_linear_cross_entropy(x, weight, target, group)
+    if z_loss_coef < 0:
+        raise ValueError(f"z_loss_coef must not be negative, got {z_loss_coef}")
+    return _LinearCrossEntropy.apply(x, weight, target, group, float(z_loss_coef))
+
+
 __all__ = [
     "column_linear",
     "row_linear",
+    "linear_cross_entropy",
+    "linear_cross_entropy_with_z_loss",
     "sharded_cross_entropy",
     "sharded_cross_entropy_with_z_loss",
     "differentiable_identity",
