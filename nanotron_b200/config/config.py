@@ -251,6 +251,9 @@ class KernelArgs:
     # operand precision of the linear-layer products: "bf16", or "fp8" = block-scaled fp8 (1 x 128 / 128 x 128 blocks, e4m3
     # forward, e5m2 gradients) for every tensor-parallel linear whose dimensions are multiples of 128
     linear: str = "bf16"
+    # what a training step keeps between the head's forward and backward: "logits" (tokens x vocabulary), or "fused" = nothing of that
+    # size (``linear_cross_entropy``: the scores stay on chip and are computed again, piece by piece, in the backward pass)
+    loss: str = "logits"
 
 
 @dataclass
@@ -326,6 +329,13 @@ class AdamWOptimizerArgs:
     adam_beta2: float
     torch_adam_is_fused: bool
     name: str = "adamW"
+    # 8: both running averages in 8-bit blocks (``FusedAdamW(state_bits=8)``), a quarter of the optimizer state's memory; the
+    # data-parallel step then goes through the collectives (the fused NVLink step keeps fp32 averages)
+    state_bits: int = 32
+
+    def __post_init__(self):
+        if self.state_bits not in (8, 32):
+            raise ValueError(f"optimizer_factory.state_bits is 8 or 32, got {self.state_bits}")
 
 
 @dataclass

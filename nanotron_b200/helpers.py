@@ -162,9 +162,9 @@ def init_optimizer_and_grad_accumulator(parametrization_method: ParametrizationM
             def optimizer(param_groups):
                 first = param_groups[0]["params"][0] if param_groups and param_groups[0]["params"] else None
                 use_native = first is not None and first.is_cuda and first.dtype == torch.float32
-                if use_native or not factory.torch_adam_is_fused:
-                    if use_native or first is None or first.dtype == torch.float32:
-                        return FusedAdamW(param_groups, lr=optimizer_args.learning_rate_scheduler.learning_rate, weight_decay=optimizer_args.weight_decay, eps=factory.adam_eps, betas=(factory.adam_beta1, factory.adam_beta2))
+                if use_native or not factory.torch_adam_is_fused or factory.state_bits == 8:
+                    if use_native or first is None or first.dtype == torch.float32 or factory.state_bits == 8:
+                        return FusedAdamW(param_groups, lr=optimizer_args.learning_rate_scheduler.learning_rate, weight_decay=optimizer_args.weight_decay, eps=factory.adam_eps, betas=(factory.adam_beta1, factory.adam_beta2), state_bits=factory.state_bits)
                 return torch.optim.AdamW(param_groups, lr=optimizer_args.learning_rate_scheduler.learning_rate, weight_decay=optimizer_args.weight_decay, eps=factory.adam_eps, betas=(factory.adam_beta1, factory.adam_beta2), fused=factory.torch_adam_is_fused and first is not None and first.is_cuda)
 
         elif factory.name == "sgd":

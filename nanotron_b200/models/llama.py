@@ -213,5 +213,6 @@ class LlamaForTraining(_q.Qwen2ForTraining):
     model_class = LlamaModel
 
     def forward(self, input_ids, input_mask, label_ids, label_mask) -> Dict[str, Union[torch.Tensor, TensorPointer]]:
-        sharded_logits = self.model(input_ids=input_ids, input_mask=input_mask)
+        with _q.head_feeds_loss(self.model.lm_head, self.loss):
+            sharded_logits = self.model(input_ids=input_ids, input_mask=input_mask)
         return self.loss(sharded_logits=sharded_logits, label_ids=label_ids, label_mask=label_mask)

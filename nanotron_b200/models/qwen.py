@@ -11,6 +11,7 @@ fused (residual add +) RMSNorm -> qkv GEMM -> in-place RoPE on the q/k views -> 
 """
 from __future__ import annotations
 
+from contextlib import contextmanager
 from typing import Dict, List, Optional, Union
 
 import torch
@@ -32,8 +33,9 @@ from nanotron_b200.parallel.parameters import NanotronParameter
 from nanotron_b200.parallel.pipeline_parallel.block import PipelineBlock, TensorPointer
 from nanotron_b200.parallel.pipeline_parallel.p2p import P2P
 from nanotron_b200.parallel.tensor_parallel.enum import TensorParallelLinearMode
-from nanotron_b200.parallel.tensor_parallel.functional import sharded_cross_entropy, sharded_cross_entropy_with_z_loss
+from nanotron_b200.parallel.tensor_parallel.functional import linear_cross_entropy, linear_cross_entropy_with_z_loss, sharded_cross_entropy, sharded_cross_entropy_with_z_loss
 from nanotron_b200.parallel.tensor_parallel.nn import (
+    DeferredLogits,
     TensorParallelColumnLinear,
     TensorParallelEmbedding,
     TensorParallelRowLinear,
@@ -316,14 +318,33 @@ def masked_mean(loss, label_mask, dtype):
     return (loss * label_mask).sum(dtype=dtype) / label_mask.sum().clamp(min=1)
 
 
+@contextmanager
+def head_feeds_loss(head: PipelineBlock, loss: PipelineBlock):
+    """Inside: the head may hand its operands to the loss instead of the logits (``ops.set_loss("fused")``), if this pipeline stage runs
+    both (logits that travel to another stage have to exist)."""
+    block = getattr(head, "pp_block", None)
+    if block is None or head.rank != loss.rank:
+        yield
+        return
+    block.feeds_loss = True
+    try:
+        yield
+    finally:
+        block.feeds_loss = False
+
+
 class Loss(nn.Module):
     def __init__(self, tp_pg: dist.ProcessGroup):
         super().__init__()
         self.tp_pg = tp_pg
 
     def forward(self, sharded_logits: torch.Tensor, label_ids: torch.Tensor, label_mask: torch.Tensor) -> Dict[str, torch.Tensor]:
-        """sharded_logits: [b*s, V/tp]; label_ids/label_mask: [b, s]."""
-        loss = sharded_cross_entropy(sharded_logits, label_ids.reshape(-1).contiguous(), group=self.tp_pg, dtype=torch.float)
+        """sharded_logits: [b*s, V/tp], or the head's operands (``DeferredLogits``); label_ids/label_mask: [b, s]."""
+        labels = label_ids.reshape(-1).contiguous()
+        if isinstance(sharded_logits, DeferredLogits):
+            loss = linear_cross_entropy(sharded_logits.x, sharded_logits.weight, labels, group=self.tp_pg)
+        else:
+            loss = sharded_cross_entropy(sharded_logits, labels, group=self.tp_pg, dtype=torch.float)
         return {"loss": masked_mean(loss, label_mask.reshape(-1), dtype=torch.float)}
 
 
@@ -333,7 +354,11 @@ class LossWithZLoss(Loss):
         self.z_loss_coef = z_loss_coefficient
 
     def forward(self, sharded_logits, label_ids, label_mask):
-        loss, z = sharded_cross_entropy_with_z_loss(sharded_logits, label_ids.reshape(-1).contiguous(), group=self.tp_pg, dtype=torch.float, z_loss_coef=self.z_loss_coef)
+        labels = label_ids.reshape(-1).contiguous()
+        if isinstance(sharded_logits, DeferredLogits):
+            loss, z = linear_cross_entropy_with_z_loss(sharded_logits.x, sharded_logits.weight, labels, group=self.tp_pg, z_loss_coef=self.z_loss_coef)
+        else:
+            loss, z = sharded_cross_entropy_with_z_loss(sharded_logits, labels, group=self.tp_pg, dtype=torch.float, z_loss_coef=self.z_loss_coef)
         m = label_mask.reshape(-1)
         z_loss = masked_mean(z.detach(), m, dtype=torch.float)
         return {"loss": masked_mean(loss + z, m, dtype=torch.float), "z_loss": z_loss}
@@ -384,7 +409,8 @@ class Qwen2ForTraining(NanotronModel):
         self.parallel_config = parallel_config
 
     def forward(self, input_ids, position_ids, label_ids, label_mask) -> Dict[str, Union[torch.Tensor, TensorPointer]]:
-        out = self.model(input_ids=input_ids, position_ids=position_ids)
+        with head_feeds_loss(self.model.lm_head, self.loss):
+            out = self.model(input_ids=input_ids, position_ids=position_ids)
         if self.is_moe:
             logits, aux = out
             return self.loss(sharded_logits=logits, label_ids=label_ids, label_mask=label_mask, aux_loss=aux)

@@ -26,7 +26,7 @@ from nanotron_b200 import ops
 from nanotron_b200.config import ParallelismArgs, Starcoder2Config
 from nanotron_b200.generation.generate_store import AttachableStore
 from nanotron_b200.models.base import NanotronModel
-from nanotron_b200.models.qwen import Loss, Qwen2ForTraining, get_flops
+from nanotron_b200.models.qwen import Loss, Qwen2ForTraining, get_flops, head_feeds_loss
 from nanotron_b200.nn.activations import ACT2FN
 from nanotron_b200.nn.attention import regular_cu_seqlens
 from nanotron_b200.nn.layer_norm import TritonLayerNorm
@@ -337,7 +337,8 @@ class Starcoder2ForTraining(NanotronModel):
         self.config, self.parallel_config, self.parallel_context = config, parallel_config, parallel_context
 
     def forward(self, input_ids, input_mask, label_ids, label_mask):
-        logits = self.model(input_ids=input_ids, input_mask=input_mask)
+        with head_feeds_loss(self.model.lm_head, self.loss):
+            logits = self.model(input_ids=input_ids, input_mask=input_mask)
         return {"loss": self.loss(sharded_logits=logits, label_ids=label_ids, label_mask=label_mask)["loss"]}
 
     def tie_custom_params(self) -> None:

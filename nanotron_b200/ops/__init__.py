@@ -20,6 +20,7 @@ _MODE = os.environ.get("NTB_OPS", "auto")  # auto | torch
 _GEMM = os.environ.get("NTB_GEMM", "auto")  # auto | cublas | tcgen05
 _ATTN = os.environ.get("NTB_ATTN", "auto")  # auto | native (both: the in-tree tcgen05 kernels) | sdpa (library kernel, for comparison)
 _LINEAR = os.environ.get("NTB_LINEAR", "bf16")  # bf16 | fp8 (block-scaled e4m3 forward / e5m2 gradients for the linear-layer products)
+_LOSS = os.environ.get("NTB_LOSS", "logits")  # logits | fused (training heads hand their operands to the loss: linear_cross_entropy)
 LAUNCH_COUNTER = {"n": 0}
 
 
@@ -52,6 +53,20 @@ def set_linear(mode: str):
 
 def get_linear() -> str:
     return _LINEAR
+
+
+def set_loss(mode: str):
+    """How a training model's head and loss work together: "logits" (the head's product is materialised and kept for backward) or "fused"
+    (``linear_cross_entropy``).  Heads that the kernels have no form for (on CUDA: not bf16, hidden size not a multiple of 64, with a
+    bias) and pipeline stages that hold the head without the loss keep the logits."""
+    global _LOSS
+    if mode not in ("logits", "fused"):
+        raise ValueError(f"loss is 'logits' or 'fused', got {mode!r}")
+    _LOSS = mode
+
+
+def get_loss() -> str:
+    return _LOSS
 
 
 def get_mode() -> str:
@@ -363,6 +378,12 @@ def ce_backward(logits2, target, logz, grad_loss, grad_z, vocab_start: int):
 
 
 # ============================================================================ cross entropy of a linear head (no logits)
+def linear_ce_supported(x: torch.Tensor, weight: torch.Tensor) -> bool:
+    if not x.is_cuda or _MODE == "torch":
+        return x.dtype == weight.dtype
+    return x.dtype == weight.dtype == torch.bfloat16 and weight.shape[1] % 64 == 0
+
+
 def linear_ce_forward(x2: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, vocab_start: int, finish: bool):
     """Softmax statistics of the scores ``x2 @ weight.T`` ([T, H], [V, H]), which are never materialised.  ``finish`` (``weight`` is the
     whole vocabulary): (logZ, loss) per token; otherwise the shard's (max, sum exp, target score or 0) like ``ce_partials``."""
@@ -637,6 +658,104 @@ def fused_qkv_library_attention(qkv, cos_table, sin_table, positions, n_heads, n
     scale = softmax_scale if softmax_scale is not None else 1.0 / math.sqrt(head_dim)
     pos = positions.to(torch.int64).contiguous() if positions is not None else None
     return _FusedQKVAttentionLib.apply(qkv, cos_table, sin_table, pos, n_heads, n_kv, head_dim, batch, seqlen, scale, interleaved, use_rope)
+
+
+# ============================================================================ optimizer step over lists of tensors
+def q8_decode(codes: torch.Tensor, exponents: torch.Tensor, signed: bool, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """The values of an 8-bit state (``adamw_multi_tensor``): uint8 codes and one uint8 exponent per 128 of them; fp32 or bf16, both exact.
+    ``signed``: the layout of ``exp_avg``; otherwise the one of ``exp_avg_sq``."""
+    _check_q8(codes, exponents, "q8_decode")
+    if dtype not in (torch.float32, torch.bfloat16):
+        raise ValueError(f"q8_decode gives float32 or bfloat16, not {dtype}")
+    if _use_native(codes):
+        from nanotron_b200.ops import native
+
+        return native.q8_decode(codes, exponents, signed, dtype)
+    return ref.q8_decode(codes, exponents, signed, dtype)
+
+
+def q8_encode(x: torch.Tensor, signed: bool):
+    """fp32 values -> (codes, exponents), rounded to the nearest code; what ``q8_decode`` returned is encoded without loss."""
+    if x.dtype != torch.float32:
+        raise ValueError(f"q8_encode takes float32, got {x.dtype}")
+    if _use_native(x):
+        from nanotron_b200.ops import native
+
+        return native.q8_encode(x.contiguous(), signed)
+    return ref.q8_encode(x, signed)
+
+
+def _check_q8(codes, exponents, what):
+    n = (codes.numel() + 127) // 128
+    if codes.dtype != torch.uint8 or exponents.dtype != torch.uint8 or exponents.numel() != n or codes.device != exponents.device or not (codes.is_contiguous() and exponents.is_contiguous()):
+        raise ValueError(f"{what}: contiguous uint8 codes and {n} uint8 exponents on the same device expected, got {tuple(codes.shape)} {codes.dtype} on {codes.device} and "
+                         f"{tuple(exponents.shape)} {exponents.dtype} on {exponents.device}")
+
+
+@torch.no_grad()
+def adamw_multi_tensor(params, grads, exp_avgs, exp_avg_sqs, *, lr, beta1: float, beta2: float, eps: float, weight_decay, step: float, halves=None,
+                       exp_avg_exponents=None, exp_avg_sq_exponents=None, grad_scale: Optional[torch.Tensor] = None, seed: int = 0) -> None:
+    """One AdamW step (decoupled decay, bias correction; ``torch.optim.AdamW``) over lists of tensors on one device, in place, in one
+    launch on CUDA.
+
+    ``params``, ``grads``: fp32 or bf16, any sizes, params contiguous.  ``lr``, ``weight_decay``: a number, or one per tensor.  ``step``: 1 for
+    the first.  ``halves``: optional bf16 tensors (or None per entry) that receive the rounded parameters.  ``grad_scale``: optional fp32
+    device scalar multiplied into every gradient (a clipping coefficient).
+
+    States: fp32 tensors of the parameters' sizes; or, with ``exp_avg_exponents`` and ``exp_avg_sq_exponents``, uint8 codes of the
+    parameters' sizes with one uint8 exponent per 128 consecutive elements (all zero: a fresh state).  8-bit states are rounded
+    stochastically by a hash of (``seed``, position of the tensor in the list, element): pass another ``seed`` every step.  Each
+    keeps 3 mantissa bits; magnitudes more than 2^15 (first moment) or 2^31 (second) below their block's largest are lost (become
+    zero) or raised to that limit.  A gradient that is not finite makes the state of its block of 128 elements NaN."""
+    n = len(params)
+    if not (len(grads) == len(exp_avgs) == len(exp_avg_sqs) == n) or any(x is not None and len(x) != n for x in (halves, exp_avg_exponents, exp_avg_sq_exponents)):
+        raise ValueError("adamw_multi_tensor: the lists have different lengths")
+    if (exp_avg_exponents is None) != (exp_avg_sq_exponents is None):
+        raise ValueError("adamw_multi_tensor: 8-bit states need the exponents of both averages")
+    if not step >= 1:
+        raise ValueError(f"adamw_multi_tensor: step counts from 1, got {step}")
+    if not (0 <= beta1 < 1 and 0 <= beta2 < 1 and eps >= 0):
+        raise ValueError(f"adamw_multi_tensor: betas in [0, 1) and eps >= 0 expected, got {beta1}, {beta2}, {eps}")
+    lrs = [float(x) for x in lr] if isinstance(lr, (list, tuple)) else [float(lr)] * n
+    wds = [float(x) for x in weight_decay] if isinstance(weight_decay, (list, tuple)) else [float(weight_decay)] * n
+    if len(lrs) != n or len(wds) != n:
+        raise ValueError("adamw_multi_tensor: one learning rate and weight decay per tensor (or one for all) expected")
+    if n == 0:
+        return
+    dev, eight = params[0].device, exp_avg_exponents is not None
+    if grad_scale is not None and (grad_scale.dtype != torch.float32 or grad_scale.numel() != 1 or grad_scale.device != dev):
+        raise ValueError("adamw_multi_tensor: grad_scale is one float32 on the parameters' device")
+    state_type = torch.uint8 if eight else torch.float32
+    floats = (torch.float32, torch.bfloat16)
+    addresses = set()
+    for i, p in enumerate(params):
+        g, m, v, size = grads[i], exp_avgs[i], exp_avg_sqs[i], p.numel()
+        if p.dtype not in floats or g.dtype not in floats or m.dtype != state_type or v.dtype != state_type:
+            raise ValueError(f"adamw_multi_tensor: tensor {i}: parameters and gradients in float32 or bfloat16 and states in {state_type} expected, got {p.dtype}, {g.dtype}, {m.dtype}, {v.dtype}")
+        if g.numel() != size or m.numel() != size or v.numel() != size:
+            raise ValueError(f"adamw_multi_tensor: tensor {i}: sizes differ: {size}, {g.numel()}, {m.numel()}, {v.numel()}")
+        if g.device != dev or p.device != dev or m.device != dev or v.device != dev:
+            raise ValueError(f"adamw_multi_tensor: tensor {i}: everything has to be on {dev}")
+        if not (p.is_contiguous() and m.is_contiguous() and v.is_contiguous()):
+            raise ValueError(f"adamw_multi_tensor: tensor {i}: parameters and states have to be contiguous")
+        if eight:
+            _check_q8(m, exp_avg_exponents[i], f"adamw_multi_tensor: tensor {i}")
+            _check_q8(v, exp_avg_sq_exponents[i], f"adamw_multi_tensor: tensor {i}")
+        h = halves[i] if halves is not None else None
+        if h is not None and (h.dtype != torch.bfloat16 or h.numel() != size or h.device != dev or not h.is_contiguous()):
+            raise ValueError(f"adamw_multi_tensor: tensor {i}: its half is a contiguous bfloat16 tensor of {size} elements on {dev}")
+        if size:
+            addresses.add(p.data_ptr())
+    if len(addresses) != sum(p.numel() > 0 for p in params):
+        raise ValueError("adamw_multi_tensor: the same parameter twice")
+    args = (params, grads, exp_avgs, exp_avg_sqs, lrs, beta1, beta2, eps, wds, step, halves, exp_avg_exponents, exp_avg_sq_exponents, grad_scale, seed)
+    if _use_native(params[0]):
+        from nanotron_b200.ops import native
+
+        native.adamw_multi(*args)
+    else:
+        ref.adamw_multi_tensor(*args)
+    torch.autograd.graph.increment_version([p for p in params if p.is_leaf or not p.requires_grad] + [h for h in halves or () if h is not None])
 
 
 from nanotron_b200.ops import tp_fused  # noqa: E402,F401

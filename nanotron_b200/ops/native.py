@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 from ctypes import c_float, c_int, c_int64, c_void_p
 from pathlib import Path
 from typing import List, Optional, Tuple
@@ -49,6 +50,12 @@ def _declare(L):
     L.ntb_ce_partials.argtypes = [c_int] + [c_void_p] * 5 + [c_int64, c_int, c_int64, c_void_p]
     L.ntb_ce_backward.argtypes = [c_int] + [c_void_p] * 6 + [c_int64, c_int, c_int64, c_void_p]
     L.ntb_adamw_flat.argtypes = [c_void_p] * 5 + [c_int64] + [c_void_p] * 3 + [c_int] + [c_float] * 5 + [c_void_p, c_void_p]
+    L.ntb_adamw_multi.restype = c_int
+    L.ntb_adamw_multi.argtypes = [c_void_p, c_int, c_int, c_int, c_int] + [c_float] * 7 + [c_void_p, c_int, c_void_p]
+    L.ntb_q8_decode.restype = c_int
+    L.ntb_q8_decode.argtypes = [c_void_p, c_void_p, c_void_p, c_int64, c_int, c_int, c_void_p]
+    L.ntb_q8_encode.restype = c_int
+    L.ntb_q8_encode.argtypes = [c_void_p, c_void_p, c_void_p, c_int64, c_int, c_void_p]
     L.ntb_sumsq_num_partials.restype = c_int
     L.ntb_sumsq.argtypes = [c_void_p, c_int64, c_void_p, c_void_p, c_int, c_void_p]
     if hasattr(L, "ntb_symm_barrier"):
@@ -235,23 +242,53 @@ def adamw_flat(p, g, m, v, p16, seg_end, seg_lr, seg_wd, beta1, beta2, eps, step
     _check(rc, "adamw_flat")
 
 
-def multi_tensor_adamw(ps, gs, ms, vs, halves, lr, beta1, beta2, eps, weight_decay, step):
-    """Per-tensor launches of the flat kernel (used when the tensors are not one contiguous range)."""
-    dev = ps[0].device
-    for p, g, m, v, h in zip(ps, gs, ms, vs, halves):
-        n = p.numel()
-        pad_ok = n % 4 == 0 and all(t.data_ptr() % 16 == 0 for t in (p, g, m, v)) and (h is None or (h.dtype == torch.bfloat16 and h.data_ptr() % 8 == 0))
-        if not pad_ok or not g.is_contiguous() or g.dtype != torch.float32:
-            from nanotron_b200.ops import reference as ref
+_AM_RECORD = struct.Struct("@7Qq2f2I")  # AmTensor of csrc/optim_multi.cu
 
-            ref.adamw_step(p, g.float(), m, v, lr, beta1, beta2, eps, weight_decay, step)
-            if h is not None:
-                h.copy_(p.view(-1))
+
+def adamw_multi(params, grads, exp_avgs, exp_avg_sqs, lrs, beta1, beta2, eps, weight_decays, step, halves, exp_avg_exponents, exp_avg_sq_exponents, grad_scale, seed):
+    """One launch for all tensors (one per pair of parameter and gradient type, and per 384 tensors).  The addresses travel as kernel
+    parameters, so nothing is copied to the device."""
+    from nanotron_b200.ops import native_gemm
+    from nanotron_b200.ops.reference import q8_tensor_key
+
+    dev = params[0].device
+    eight = exp_avg_exponents is not None
+    bc1, bc2 = 1.0 - beta1**step, 1.0 - beta2**step
+    records, kept = {}, []
+    for i, (p, g, m, v) in enumerate(zip(params, grads, exp_avgs, exp_avg_sqs)):
+        n = p.numel()
+        if n == 0:
             continue
-        seg_end = torch.tensor([n], dtype=torch.int64, device=dev)
-        seg_lr = torch.tensor([lr], dtype=torch.float32, device=dev)
-        seg_wd = torch.tensor([weight_decay], dtype=torch.float32, device=dev)
-        adamw_flat(p.view(-1), g.view(-1), m.view(-1), v.view(-1), h, seg_end, seg_lr, seg_wd, beta1, beta2, eps, step)
+        if not g.is_contiguous():
+            g = g.contiguous()
+            kept.append(g)
+        h = halves[i] if halves is not None else None
+        records.setdefault((p.dtype, g.dtype), []).append(
+            _AM_RECORD.pack(p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), 0 if h is None else h.data_ptr(), exp_avg_exponents[i].data_ptr() if eight else 0,
+                            exp_avg_sq_exponents[i].data_ptr() if eight else 0, n, lrs[i], weight_decays[i], q8_tensor_key(seed, i) if eight else 0, 0))
+    L = lib()
+    with torch.cuda.device(dev):
+        for (pt, gt), rows in records.items():
+            table = ctypes.create_string_buffer(b"".join(rows), len(rows) * _AM_RECORD.size)
+            _check(L.ntb_adamw_multi(table, len(rows), _DT[pt], _DT[gt], 8 if eight else 32, beta1, 1.0 - beta1, beta2, 1.0 - beta2, eps, bc1, bc2, _ptr(grad_scale),
+                                     native_gemm._sms(dev), _stream(params[0])), "adamw_multi")
+
+
+def q8_decode(codes, exponents, signed: bool, dtype):
+    out = torch.empty(codes.shape, dtype=dtype, device=codes.device)
+    if codes.numel():
+        with torch.cuda.device(codes.device):
+            _check(lib().ntb_q8_decode(codes.data_ptr(), exponents.data_ptr(), out.data_ptr(), codes.numel(), int(signed), _DT[dtype], _stream(codes)), "q8_decode")
+    return out
+
+
+def q8_encode(x, signed: bool):
+    codes = torch.empty(x.shape, dtype=torch.uint8, device=x.device)
+    exponents = torch.empty((x.numel() + 127) // 128, dtype=torch.uint8, device=x.device)
+    if x.numel():
+        with torch.cuda.device(x.device):
+            _check(lib().ntb_q8_encode(x.data_ptr(), codes.data_ptr(), exponents.data_ptr(), x.numel(), int(signed), _stream(x)), "q8_encode")
+    return codes, exponents
 
 
 def sumsq(x: torch.Tensor, out: Optional[torch.Tensor] = None, accumulate: bool = False) -> torch.Tensor:

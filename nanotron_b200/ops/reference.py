@@ -249,3 +249,90 @@ def adamw_step(p, g, m, v, lr, beta1, beta2, eps, weight_decay, step, grad_scale
     bc2 = 1 - beta2**step
     denom = (v.sqrt() / math.sqrt(bc2)).add_(eps)
     p.addcdiv_(m, denom, value=-lr / bc1)
+
+
+# ------------------------------------------------------------------ optimizer states in 8-bit blocks
+Q8_BLOCK = 128
+
+
+def mix32(x):
+    """A 32-bit mixing function (xor-shift and multiply, twice; C. Wellons' published low-bias constants) of Python integers or int64
+    tensors below 2^32."""
+    x = ((x ^ (x >> 16)) * 0x7FEB352D) & 0xFFFFFFFF
+    x = ((x ^ (x >> 15)) * 0x846CA68B) & 0xFFFFFFFF
+    return x ^ (x >> 16)
+
+
+def q8_tensor_key(seed: int, index: int) -> int:
+    """Key of the random bits of a call's tensor number ``index``."""
+    return mix32((seed + 0x9E3779B9 * (index + 1)) & 0xFFFFFFFF)
+
+
+def q8_random_bits(n: int, key: int, device=None) -> torch.Tensor:
+    """32 random bits (int64) for each of a tensor's ``n`` elements."""
+    i = torch.arange(n, dtype=torch.int64, device=device)
+    return mix32((i & 0xFFFFFFFF) ^ ((key + (i >> 32) * 0x9E3779B9) & 0xFFFFFFFF))
+
+
+def _q8_blocks(x: torch.Tensor) -> torch.Tensor:
+    return F.pad(x.reshape(-1), (0, -x.numel() % Q8_BLOCK)).view(-1, Q8_BLOCK)
+
+
+def q8_encode(x: torch.Tensor, signed: bool, bits16: Optional[torch.Tensor] = None):
+    """fp32 values -> (codes uint8 of x's shape, exponents uint8 [ceil(n / 128)]).
+
+    128 consecutive elements share the fp32 exponent field E of their largest magnitude.  Code c > 0 counts eighths of binades from
+    the lower end of the window below 2^(E - 127): a sign and 7 bits (15 binades) for ``signed``, else 8 bits (31 binades).  The cut 20
+    mantissa bits round up where they and ``bits16`` (16 random bits per element; default: to nearest) carry.  Signed values below
+    the window become 0, unsigned ones its smallest code.  A block with a value that is not finite gets E = 255 (NaN throughout)."""
+    top = 127 if signed else 255
+    raw = _q8_blocks(x.float()).contiguous().view(torch.int32).to(torch.int64)
+    size = raw & 0x7FFFFFFF
+    e = (size >> 23).amax(dim=1, keepdim=True)
+    share = torch.full_like(size, 0x8000) if bits16 is None else _q8_blocks(bits16)
+    c = (((size + (share << 4) + 8) >> 20) - 8 * e + (top - 7)).clamp(0 if signed else 1, top)
+    c = torch.where((size < 1 << 23) | (e == 255), torch.zeros_like(c), c)
+    if signed:
+        c = torch.where((c > 0) & (raw < 0), c + 128, c)
+    return c.view(-1)[: x.numel()].to(torch.uint8).view(x.shape), e.view(-1).to(torch.uint8)
+
+
+def q8_decode(codes: torch.Tensor, exponents: torch.Tensor, signed: bool, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """The values of ``q8_encode``'s codes (four significant bits and a power of two: exact in bf16)."""
+    top = 127 if signed else 255
+    c, e = _q8_blocks(codes).to(torch.int64), exponents.to(torch.int64).unsqueeze(1)
+    size = (c & top) + 8 * e - (top - 7)
+    size = torch.where(((c & top) == 0) | (size < 8), torch.zeros_like(size), size)
+    x = (size << 20).to(torch.int32).view(torch.float32)
+    x = torch.where(c > top, -x, x)
+    x = torch.where(e == 255, torch.full_like(x, float("nan")), x)
+    return x.view(-1)[: codes.numel()].view(codes.shape).to(dtype)
+
+
+def adamw_multi_tensor(params, grads, exp_avgs, exp_avg_sqs, lrs, beta1, beta2, eps, weight_decays, step, halves, exp_avg_exponents, exp_avg_sq_exponents, grad_scale, seed):
+    """One AdamW step over lists of tensors, in place (see ``ops.adamw_multi_tensor``).  Every operation is rounded to fp32 by itself."""
+    bc1, bc2 = 1 - beta1**step, 1 - beta2**step
+    for i, (p, g, ms, vs) in enumerate(zip(params, grads, exp_avgs, exp_avg_sqs)):
+        if p.numel() == 0:
+            continue
+        eight = exp_avg_exponents is not None
+        m = q8_decode(ms, exp_avg_exponents[i], True) if eight else ms
+        v = q8_decode(vs, exp_avg_sq_exponents[i], False) if eight else vs
+        g = g.float().reshape(m.shape)
+        if grad_scale is not None:
+            g = g * grad_scale.float().view(())
+        m = m * beta1 + g * (1 - beta1)
+        v = v * beta2 + (g * g) * (1 - beta2)
+        q = p.float() * (1 - lrs[i] * weight_decays[i]) - ((lrs[i] / bc1) * (m / (v.sqrt() * (1.0 / math.sqrt(bc2)) + eps))).view(p.shape)
+        p.copy_(q)
+        if halves is not None and halves[i] is not None:
+            halves[i].copy_(q.view(halves[i].shape))
+        if eight:
+            bits = q8_random_bits(p.numel(), q8_tensor_key(seed, i), p.device)
+            for value, r, codes, exponents, signed in ((m, bits & 0xFFFF, ms, exp_avg_exponents[i], True), (v, bits >> 16, vs, exp_avg_sq_exponents[i], False)):
+                c, e = q8_encode(value, signed, r)
+                codes.copy_(c)
+                exponents.copy_(e)
+        else:
+            ms.copy_(m)
+            vs.copy_(v)

@@ -5,7 +5,12 @@ builds) and its gradient / half-precision twin sit at a constant offset in their
 optimizer step is a single launch of the in-tree flat kernel: gradient scaling (clipping coefficient read on the
 device), AdamW, and the bf16 write-back of the updated weights, replacing the separate fp32->bf16 pass of the
 reference (reference src/nanotron/optim/gradient_accumulator.py:255-267).  The ``exp_avg`` / ``exp_avg_sq`` states
-are views of two flat buffers with the same layout.  Otherwise (CPU, or scattered tensors) it runs per tensor.
+are views of two flat buffers with the same layout.  Scattered tensors take one launch of the multi-tensor kernel
+(``ops.adamw_multi_tensor``); what that has no form for (fp16, strided parameters, bf16 states) runs per tensor.
+
+``state_bits=8`` keeps both averages as 8-bit codes with one exponent byte per 128 elements: 2.02 bytes per parameter instead
+of 8.  The state dict holds them as fp32 tensors all the same (an 8-bit value is exact there, and encoding it again gives the
+same codes), so checkpoints move freely between both forms and between layouts.
 """
 from __future__ import annotations
 
@@ -17,7 +22,11 @@ from nanotron_b200.ops import reference as ref
 
 
 class FusedAdamW(torch.optim.Optimizer):
-    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2):
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits: int = 32, state_seed: int = 0):
+        if state_bits not in (8, 32):
+            raise ValueError(f"state_bits is 8 or 32, got {state_bits}")
+        self.state_bits = state_bits
+        self.state_seed = state_seed  # of the stochastic rounding of 8-bit states; mixed with the step number
         defaults = dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay)
         super().__init__(params, defaults)
         self.half_targets: Dict[int, torch.Tensor] = {}  # id(master) -> flat half-precision destination view
@@ -34,11 +43,42 @@ class FusedAdamW(torch.optim.Optimizer):
     # ------------------------------------------------------------------ state
     def _init_state(self, p):
         st = self.state[p]
+        if self.state_bits == 8:
+            return self._init_state8(p, st)
         if len(st) == 0:
             st["step"] = torch.zeros((), dtype=torch.float32)
             st["exp_avg"] = torch.zeros_like(p, memory_format=torch.preserve_format)
             st["exp_avg_sq"] = torch.zeros_like(p, memory_format=torch.preserve_format)
         return st
+
+    def _init_state8(self, p, st):
+        if len(st) == 0:
+            st["step"] = torch.zeros((), dtype=torch.float32)
+        for key in ("exp_avg", "exp_avg_sq"):
+            if key not in st:
+                st[key] = torch.zeros(p.shape, dtype=torch.uint8, device=p.device)
+                st[key + "_exponents"] = torch.zeros((p.numel() + 127) // 128, dtype=torch.uint8, device=p.device)
+            elif st[key].dtype != torch.uint8:  # loaded from a checkpoint
+                from nanotron_b200 import ops
+
+                st[key], st[key + "_exponents"] = ops.q8_encode(st[key].to(p.device, torch.float32).contiguous().view(p.shape), signed=key == "exp_avg")
+        return st
+
+    def state_dict(self):
+        """As ``torch.optim.AdamW`` gives it; 8-bit states appear as the fp32 values they stand for."""
+        sd = super().state_dict()
+        if self.state_bits == 8:
+            from nanotron_b200 import ops
+
+            def decoded(st):
+                out = {k: v for k, v in st.items() if not k.endswith("_exponents")}
+                for key in ("exp_avg", "exp_avg_sq"):
+                    if key + "_exponents" in st and st[key].dtype == torch.uint8:
+                        out[key] = ops.q8_decode(st[key], st[key + "_exponents"], signed=key == "exp_avg")
+                return out
+
+            sd["state"] = {k: decoded(st) if isinstance(st, dict) else st for k, st in sd["state"].items()}
+        return sd
 
     def _try_build_flat_plan(self):
         """All params must tile one contiguous fp32 range in address order, with constant grad / half offsets."""
@@ -118,6 +158,9 @@ class FusedAdamW(torch.optim.Optimizer):
         from nanotron_b200 import ops
 
         first = next((p for g in self.param_groups for p in g["params"]), None)
+        if self.state_bits == 8:
+            self._step8()
+            return loss
         if first is not None and first.is_cuda and ops.get_mode() != "torch" and not self._flat_failed:
             if self._flat is None:
                 self._flat = self._try_build_flat_plan()
@@ -148,38 +191,75 @@ class FusedAdamW(torch.optim.Optimizer):
             for p, _ in plan["items"]:
                 p._half_written = True
 
+    def _step8(self):
+        """All tensors with the same hyper-parameters and step number in one call (on CUDA one launch)."""
+        from nanotron_b200 import ops
+
+        calls = {}
+        for group in self.param_groups:
+            for p in group["params"]:
+                if p.grad is None:
+                    continue
+                st = self._init_state(p)
+                st["step"] += 1
+                calls.setdefault((group["betas"], group["eps"], float(st["step"])), []).append((p, st, float(group["lr"]), float(group["weight_decay"])))
+        scale = self.grad_scale.to(torch.float32) if self.grad_scale is not None else None
+        for (betas, eps, step), items in calls.items():
+            ps = [p for p, *_ in items]
+            targets = [self.half_targets.get(id(p)) for p in ps]
+            halves = [h if h is not None and h.dtype == torch.bfloat16 and h.is_contiguous() else None for h in targets]
+            ops.adamw_multi_tensor(
+                ps, [p.grad for p in ps], [st["exp_avg"] for _, st, *_ in items], [st["exp_avg_sq"] for _, st, *_ in items],
+                exp_avg_exponents=[st["exp_avg_exponents"] for _, st, *_ in items], exp_avg_sq_exponents=[st["exp_avg_sq_exponents"] for _, st, *_ in items],
+                halves=halves, lr=[lr for *_, lr, _ in items], weight_decay=[wd for *_, wd in items], beta1=betas[0], beta2=betas[1], eps=eps, step=step,
+                grad_scale=scale, seed=ref.mix32((self.state_seed * 0x9E3779B9 + int(step)) & 0xFFFFFFFF),
+            )
+            for p, target, written in zip(ps, targets, halves):
+                if target is None:
+                    continue
+                if written is None:  # fp16 or fp32 copies
+                    target.copy_(p.view(-1))
+                p._half_written = True
+
     def _per_tensor_step(self):
         from nanotron_b200 import ops
 
         for group in self.param_groups:
             beta1, beta2 = group["betas"]
             lr = float(group["lr"])
-            ps, gs, ms, vs, halves = [], [], [], [], []
-            step_val = None
+            together, alone = {}, []  # step number -> tensors that the multi-tensor kernel takes; the others
             for p in group["params"]:
                 if p.grad is None:
                     continue
                 st = self._init_state(p)
                 st["step"] += 1
-                step_val = float(st["step"])
-                ps.append(p), gs.append(p.grad), ms.append(st["exp_avg"]), vs.append(st["exp_avg_sq"]), halves.append(self.half_targets.get(id(p)))
-            if not ps:
-                continue
-            if ps[0].is_cuda and ps[0].dtype == torch.float32 and ops.get_mode() != "torch" and self.grad_scale is None:
-                from nanotron_b200.ops import native
-
-                native.multi_tensor_adamw(ps, gs, ms, vs, halves, lr, beta1, beta2, group["eps"], group["weight_decay"], step_val)
-            else:
-                scale = float(self.grad_scale) if self.grad_scale is not None else 1.0
-                for p, g, m, v, h in zip(ps, gs, ms, vs, halves):
-                    if p.dtype == torch.float32:
-                        ref.adamw_step(p, g.float(), m, v, lr, beta1, beta2, group["eps"], group["weight_decay"], step_val, grad_scale=scale)
-                    else:
-                        pf, mf, vf = p.float(), m.float(), v.float()
-                        ref.adamw_step(pf, g.float(), mf, vf, lr, beta1, beta2, group["eps"], group["weight_decay"], step_val, grad_scale=scale)
-                        p.copy_(pf), m.copy_(mf), v.copy_(vf)
-                    if h is not None:
-                        h.copy_(p.view(-1))
-            for p, h in zip(ps, halves):
+                item = (p, p.grad, st["exp_avg"], st["exp_avg_sq"], self.half_targets.get(id(p)))
+                if p.is_cuda and ops.get_mode() != "torch" and self._multi_tensor_takes(*item):
+                    together.setdefault(float(st["step"]), []).append(item)
+                else:
+                    alone.append((float(st["step"]), item))
+            for step_val, items in together.items():
+                ps, gs, ms, vs, halves = (list(x) for x in zip(*items))
+                scale = self.grad_scale.to(torch.float32) if self.grad_scale is not None else None
+                ops.adamw_multi_tensor(ps, gs, ms, vs, lr=lr, beta1=beta1, beta2=beta2, eps=group["eps"], weight_decay=group["weight_decay"], step=step_val, halves=halves, grad_scale=scale)
+            scale = float(self.grad_scale) if alone and self.grad_scale is not None else 1.0
+            for step_val, (p, g, m, v, h) in alone:
+                if p.dtype == torch.float32:
+                    ref.adamw_step(p, g.float(), m, v, lr, beta1, beta2, group["eps"], group["weight_decay"], step_val, grad_scale=scale)
+                else:
+                    pf, mf, vf = p.float(), m.float(), v.float()
+                    ref.adamw_step(pf, g.float(), mf, vf, lr, beta1, beta2, group["eps"], group["weight_decay"], step_val, grad_scale=scale)
+                    p.copy_(pf), m.copy_(mf), v.copy_(vf)
+                if h is not None:
+                    h.copy_(p.view(-1))
+            for p, _, _, _, h in [it for items in together.values() for it in items] + [it for _, it in alone]:
                 if h is not None:
                     p._half_written = True
+
+    @staticmethod
+    def _multi_tensor_takes(p, g, m, v, h) -> bool:
+        return (
+            p.dtype == torch.float32 and g.dtype in (torch.float32, torch.bfloat16) and m.dtype == v.dtype == torch.float32
+            and p.is_contiguous() and m.is_contiguous() and v.is_contiguous() and g.device == m.device == v.device == p.device
+            and (h is None or (h.dtype == torch.bfloat16 and h.is_contiguous()))
+        )

@@ -7,6 +7,7 @@ import torch
 from torch import nn
 
 import nanotron_b200.distributed as dist
+from nanotron_b200 import ops
 from nanotron_b200.parallel.parameters import NanotronParameter
 from nanotron_b200.parallel.sharded_parameters import (
     SplitConfig,
@@ -22,6 +23,14 @@ from nanotron_b200.parallel.tensor_parallel.distributed_differentiable_primitive
 from nanotron_b200.parallel.tensor_parallel.enum import TensorParallelLinearMode
 from nanotron_b200.parallel.tensor_parallel.functional import column_linear, row_linear
 from nanotron_b200.parallel.tied_parameters import create_tied_parameter
+
+
+class DeferredLogits:
+    """A head's operands in place of its product: ``x`` [tokens, H] (gathered over the group where the tokens are sharded) and the rows of
+    the head weight that this rank holds.  The loss takes them with ``linear_cross_entropy``."""
+
+    def __init__(self, x: torch.Tensor, weight: torch.Tensor):
+        self.x, self.weight = x, weight
 
 
 class TensorParallelColumnLinear(nn.Linear):
@@ -50,11 +59,15 @@ class TensorParallelColumnLinear(nn.Linear):
         super().__init__(in_features=self.in_features, out_features=self.out_features, bias=bias, device=device, dtype=dtype)
         self.mode = mode
         self.async_communication = async_communication
+        self.feeds_loss = False  # set by a training model around its forward when this is its head and the loss runs on the same stage
         if contiguous_chunks is not None:
             assert sum(contiguous_chunks) == out_features, f"Sum of contiguous chunks ({sum(contiguous_chunks)}) must equal out_features ({out_features})"
         mark_all_parameters_in_module_as_sharded(self, pg=self.pg, split_config=SplitConfig(split_dim=0, contiguous_chunks=contiguous_chunks))
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
+        if self.feeds_loss and self.training and self.bias is None and ops.get_loss() == "fused" and ops.linear_ce_supported(x, self.weight):
+            full = differentiable_identity(x, self.pg) if self.mode is TensorParallelLinearMode.ALL_REDUCE else differentiable_all_gather(x, self.pg)
+            return {"logits": DeferredLogits(full, self.weight)}  # a head's block names its output "logits"
         return column_linear(
             input=x,
             weight=self.weight,

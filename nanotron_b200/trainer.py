@@ -110,6 +110,7 @@ class DistributedTrainer:
                 ops.set_attention(self.config.kernels.attention)
             if getattr(self.config.kernels, "linear", "bf16") in ("bf16", "fp8"):
                 ops.set_linear(self.config.kernels.linear)
+            ops.set_loss(self.config.kernels.loss)
         self.pre_init()
         if self.config.logging is None:
             from nanotron_b200.config import LoggingArgs
@@ -207,7 +208,7 @@ class DistributedTrainer:
         ctx, opt = self.parallel_context, self.config.optimizer
         if opt.fused_zero_comm is False or ctx.device.type != "cuda" or ctx.dp_pg.size() == 1:
             return None
-        if not opt.accumulate_grad_in_fp32 or opt.optimizer_factory.name != "adamW" or ctx.cp_pg.size() > 1 or ctx.expert_parallel_size > 1:
+        if not opt.accumulate_grad_in_fp32 or opt.optimizer_factory.name != "adamW" or opt.optimizer_factory.state_bits == 8 or ctx.cp_pg.size() > 1 or ctx.expert_parallel_size > 1:
             return None
         if ctx.world_size > ctx.local_world_size:
             dp_ranks = dist.get_global_ranks(ctx.dp_pg)
