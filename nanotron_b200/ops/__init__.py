@@ -384,33 +384,36 @@ def linear_ce_supported(x: torch.Tensor, weight: torch.Tensor) -> bool:
     return x.dtype == weight.dtype == torch.bfloat16 and weight.shape[1] % 64 == 0
 
 
-def linear_ce_forward(x2: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, vocab_start: int, finish: bool):
+def linear_ce_forward(x2: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, vocab_start: int, finish: bool, z_coef: float = 0.0):
     """Softmax statistics of the scores ``x2 @ weight.T`` ([T, H], [V, H]), which are never materialised.  ``finish`` (``weight`` is the
-    whole vocabulary): (logZ, loss) per token; otherwise the shard's (max, sum exp, target score or 0) like ``ce_partials``."""
+    whole vocabulary): (logZ, loss, z_coef logZ^2 or None) per token; otherwise the shard's (max, sum exp, target score or 0) like
+    ``ce_partials``."""
     if _use_native(x2):
         from nanotron_b200.ops import native_ce
 
         native_ce.check_operands(x2, weight, target)
-        return native_ce.forward(x2, weight, target, vocab_start, finish)
+        out = native_ce.forward(x2, weight, target, vocab_start, finish, z_coef).unbind(0)
+        return out if len(out) == 3 else (*out, None)
     m, s, t = ref.linear_ce_partials(x2, weight, target, vocab_start)
     if not finish:
         return m, s, t
     logz = m + torch.log(s)
-    return logz, logz - t
+    return logz, logz - t, (z_coef * logz.square() if z_coef > 0 else None)
 
 
-def linear_ce_backward(x2, weight, target, logz, grad_loss, grad_z, vocab_start: int, need_dx: bool = True, need_dw: bool = True):
-    """(dx, dw) of the losses.  A weight that carries an fp32 ``main_grad`` gets its gradient added there, and None is returned for it."""
+def linear_ce_backward(x2, weight, target, logz, grad_loss, grad_z, z_coef: float, vocab_start: int, need_dx: bool = True, need_dw: bool = True):
+    """(dx, dw) for the upstream gradients of the losses and of the terms z_coef logZ^2 (or None).  A weight that carries an fp32
+    ``main_grad`` gets its gradient added there, and None is returned for it."""
     main_grad = getattr(weight, "main_grad", None) if need_dw else None
     if _use_native(x2):
         from nanotron_b200.ops import native_ce
 
         direct = main_grad is not None and main_grad.dtype == torch.float32 and main_grad.stride(1) == 1 and main_grad.stride(0) % 8 == 0 and main_grad.data_ptr() % 16 == 0
-        dx, dw = native_ce.backward(x2, weight, target, logz, grad_loss, grad_z, vocab_start, need_dx, need_dw, main_grad if direct else None)
+        dx, dw = native_ce.backward(x2, weight, target, logz, grad_loss, grad_z, z_coef, vocab_start, need_dx, need_dw, main_grad if direct else None)
         if direct:
             return dx, None
     else:
-        dx, dw = ref.linear_ce_backward(x2, weight, target, logz, grad_loss, grad_z, vocab_start)
+        dx, dw = ref.linear_ce_backward(x2, weight, target, logz, grad_loss, grad_z, z_coef, vocab_start)
     if main_grad is not None:
         main_grad.add_(dw)
         dw = None
@@ -707,55 +710,62 @@ def adamw_multi_tensor(params, grads, exp_avgs, exp_avg_sqs, *, lr, beta1: float
     stochastically by a hash of (``seed``, position of the tensor in the list, element): pass another ``seed`` every step.  Each
     keeps 3 mantissa bits; magnitudes more than 2^15 (first moment) or 2^31 (second) below their block's largest are lost (become
     zero) or raised to that limit.  A gradient that is not finite makes the state of its block of 128 elements NaN."""
-    n = len(params)
+    n, eight = len(params), exp_avg_exponents is not None
     if not (len(grads) == len(exp_avgs) == len(exp_avg_sqs) == n) or any(x is not None and len(x) != n for x in (halves, exp_avg_exponents, exp_avg_sq_exponents)):
         raise ValueError("adamw_multi_tensor: the lists have different lengths")
-    if (exp_avg_exponents is None) != (exp_avg_sq_exponents is None):
+    if eight != (exp_avg_sq_exponents is not None):
         raise ValueError("adamw_multi_tensor: 8-bit states need the exponents of both averages")
     if not step >= 1:
         raise ValueError(f"adamw_multi_tensor: step counts from 1, got {step}")
     if not (0 <= beta1 < 1 and 0 <= beta2 < 1 and eps >= 0):
         raise ValueError(f"adamw_multi_tensor: betas in [0, 1) and eps >= 0 expected, got {beta1}, {beta2}, {eps}")
-    lrs = [float(x) for x in lr] if isinstance(lr, (list, tuple)) else [float(lr)] * n
-    wds = [float(x) for x in weight_decay] if isinstance(weight_decay, (list, tuple)) else [float(weight_decay)] * n
-    if len(lrs) != n or len(wds) != n:
-        raise ValueError("adamw_multi_tensor: one learning rate and weight decay per tensor (or one for all) expected")
+    if isinstance(lr, (list, tuple)) or isinstance(weight_decay, (list, tuple)):
+        lr = [float(x) for x in lr] if isinstance(lr, (list, tuple)) else [float(lr)] * n
+        weight_decay = [float(x) for x in weight_decay] if isinstance(weight_decay, (list, tuple)) else [float(weight_decay)] * n
+        if len(lr) != n or len(weight_decay) != n:
+            raise ValueError("adamw_multi_tensor: one learning rate and weight decay per tensor (or one for all) expected")
+    else:
+        lr, weight_decay = float(lr), float(weight_decay)
     if n == 0:
         return
-    dev, eight = params[0].device, exp_avg_exponents is not None
+    dev = params[0].device
     if grad_scale is not None and (grad_scale.dtype != torch.float32 or grad_scale.numel() != 1 or grad_scale.device != dev):
         raise ValueError("adamw_multi_tensor: grad_scale is one float32 on the parameters' device")
-    state_type = torch.uint8 if eight else torch.float32
-    floats = (torch.float32, torch.bfloat16)
-    addresses = set()
-    for i, p in enumerate(params):
-        g, m, v, size = grads[i], exp_avgs[i], exp_avg_sqs[i], p.numel()
-        if p.dtype not in floats or g.dtype not in floats or m.dtype != state_type or v.dtype != state_type:
-            raise ValueError(f"adamw_multi_tensor: tensor {i}: parameters and gradients in float32 or bfloat16 and states in {state_type} expected, got {p.dtype}, {g.dtype}, {m.dtype}, {v.dtype}")
-        if g.numel() != size or m.numel() != size or v.numel() != size:
-            raise ValueError(f"adamw_multi_tensor: tensor {i}: sizes differ: {size}, {g.numel()}, {m.numel()}, {v.numel()}")
-        if g.device != dev or p.device != dev or m.device != dev or v.device != dev:
-            raise ValueError(f"adamw_multi_tensor: tensor {i}: everything has to be on {dev}")
-        if not (p.is_contiguous() and m.is_contiguous() and v.is_contiguous()):
-            raise ValueError(f"adamw_multi_tensor: tensor {i}: parameters and states have to be contiguous")
-        if eight:
-            _check_q8(m, exp_avg_exponents[i], f"adamw_multi_tensor: tensor {i}")
-            _check_q8(v, exp_avg_sq_exponents[i], f"adamw_multi_tensor: tensor {i}")
-        h = halves[i] if halves is not None else None
-        if h is not None and (h.dtype != torch.bfloat16 or h.numel() != size or h.device != dev or not h.is_contiguous()):
-            raise ValueError(f"adamw_multi_tensor: tensor {i}: its half is a contiguous bfloat16 tensor of {size} elements on {dev}")
-        if size:
-            addresses.add(p.data_ptr())
-    if len(addresses) != sum(p.numel() > 0 for p in params):
+    # whole lists at a time: for many small tensors these checks are a good part of the call
+    state_type, floats, sizes = (torch.uint8 if eight else torch.float32), {torch.float32, torch.bfloat16}, [p.numel() for p in params]
+
+    def check(what, tensors, types, numels, contiguous=True):
+        if not {t.dtype for t in tensors} <= types:
+            raise ValueError(f"adamw_multi_tensor: {what} in {sorted(map(str, types))} expected, got {sorted({str(t.dtype) for t in tensors})}")
+        if [t.numel() for t in tensors] != numels:
+            raise ValueError(f"adamw_multi_tensor: {what}: the sizes {[t.numel() for t in tensors]} do not fit, {numels} expected")
+        if {t.device for t in tensors} != {dev}:
+            raise ValueError(f"adamw_multi_tensor: {what}: everything has to be on {dev}")
+        if contiguous and not all([t.is_contiguous() for t in tensors]):
+            raise ValueError(f"adamw_multi_tensor: {what} have to be contiguous")
+
+    check("parameters", params, floats, sizes)
+    check("gradients", grads, floats, sizes, contiguous=False)
+    check("first moments", exp_avgs, {state_type}, sizes)
+    check("second moments", exp_avg_sqs, {state_type}, sizes)
+    if eight:
+        blocks = [(k + 127) // 128 for k in sizes]
+        check("first moments' exponents", exp_avg_exponents, {torch.uint8}, blocks)
+        check("second moments' exponents", exp_avg_sq_exponents, {torch.uint8}, blocks)
+    written = [h for h in halves if h is not None] if halves is not None else []
+    if written:
+        check("halves", written, {torch.bfloat16}, [k for k, h in zip(sizes, halves) if h is not None])
+    addresses = [p.data_ptr() for p, k in zip(params, sizes) if k]
+    if len(set(addresses)) != len(addresses):
         raise ValueError("adamw_multi_tensor: the same parameter twice")
-    args = (params, grads, exp_avgs, exp_avg_sqs, lrs, beta1, beta2, eps, wds, step, halves, exp_avg_exponents, exp_avg_sq_exponents, grad_scale, seed)
+    args = (params, grads, exp_avgs, exp_avg_sqs, lr, beta1, beta2, eps, weight_decay, step, halves, exp_avg_exponents, exp_avg_sq_exponents, grad_scale, seed)
     if _use_native(params[0]):
         from nanotron_b200.ops import native
 
         native.adamw_multi(*args)
+        torch.autograd.graph.increment_version([*params, *exp_avgs, *exp_avg_sqs, *written])
     else:
         ref.adamw_multi_tensor(*args)
-    torch.autograd.graph.increment_version([p for p in params if p.is_leaf or not p.requires_grad] + [h for h in halves or () if h is not None])
 
 
 from nanotron_b200.ops import tp_fused  # noqa: E402,F401

@@ -552,10 +552,9 @@ gemm2_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
 
 // Split tiles: D tile = (D tile +) the sum, in chunk order, of the tile's workspace slabs (256 x 256 fp32 each, complete once the
 // GEMM kernel has finished).  One block per split tile and 32-row group.  OUT as in the GEMM kernel.
-// `alpha`: device scalar multiplied into every sum (null: 1).
 template <int OUT>
 __global__ void gemm2_split_fixup_kernel(const float* __restrict__ ws, void* __restrict__ d_, int64_t ldd, int M, int N, int k_blocks, PSched sched, int tiles_m,
-                                         int tiles_n, int band, int m_rot, const float* __restrict__ alpha = nullptr) {
+                                         int tiles_n, int band, int m_rot) {
   const int rt = blockIdx.x >> 3, rg = blockIdx.x & 7;
   PTile tc = pair_tile(sched.full_units + rt, tiles_m, tiles_n, band);
   tc.m_blk = (tc.m_blk + m_rot) % tiles_m;
@@ -580,10 +579,6 @@ __global__ void gemm2_split_fixup_kernel(const float* __restrict__ ws, void* __r
       const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
       f[0] += a.x; f[1] += a.y; f[2] += a.z; f[3] += a.w;
       f[4] += b.x; f[5] += b.y; f[6] += b.z; f[7] += b.w;
-    }
-    if (alpha != nullptr) {  // not combined with P_OUT_F32_ACCUM
-#pragma unroll
-      for (int j = 0; j < 8; j++) f[j] *= *alpha;
     }
     if (OUT == P_OUT_BF16) {
       Vec8<__nv_bfloat16> o;

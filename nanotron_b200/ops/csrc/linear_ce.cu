@@ -22,7 +22,7 @@ constexpr int CE_JOIN_PARTS = 16;
 __global__ void __launch_bounds__(CE_JOIN_ROWS * CE_JOIN_PARTS)
 ce_join_kernel(const float2* __restrict__ part, const float* __restrict__ tgt, const int64_t* __restrict__ target, int64_t vocab_start, int vocab, int tiles,
                int rows, float* __restrict__ out_max, float* __restrict__ out_sum, float* __restrict__ out_tgt, float* __restrict__ logz,
-               float* __restrict__ loss) {
+               float* __restrict__ loss, float* __restrict__ z, float z_coef) {
   __shared__ float sm[CE_JOIN_PARTS][CE_JOIN_ROWS], ss[CE_JOIN_PARTS][CE_JOIN_ROWS];
   const int lane = threadIdx.x & 31, grp = threadIdx.x >> 5;
   const int row = blockIdx.x * CE_JOIN_ROWS + lane;
@@ -57,20 +57,22 @@ ce_join_kernel(const float2* __restrict__ part, const float* __restrict__ tgt, c
     const float lz = gm + logf(gs);
     logz[row] = lz;
     loss[row] = lz - t;
+    if (z != nullptr) z[row] = z_coef * (lz * lz);
   }
 }
 
-// coef = (g + gz) / unit, g = g / unit with unit = the largest |g| or |g + gz| (1 where that is no use as a divisor).  One block.
-__global__ void __launch_bounds__(1024) ce_row_coefficients_kernel(const float* __restrict__ g, const float* __restrict__ gz, int rows, float* __restrict__ coef,
-                                                                    float* __restrict__ gn, float* __restrict__ unit) {
+// coef = (g + 2 z_coef logz gz) / unit, g = g / unit with unit = the largest |g| or |g + 2 z_coef logz gz| (1 where that is no use as a
+// divisor).  One block: a reduction over the tokens, then a second look at values that are in the cache.
+__global__ void __launch_bounds__(1024) ce_row_coefficients_kernel(const float* __restrict__ g, const float* __restrict__ gz, const float* __restrict__ logz, float z_coef,
+                                                                    int rows, float* __restrict__ coef, float* __restrict__ gn, float* __restrict__ unit) {
   __shared__ float scratch[32];
   float m = 0.f;
-  for (int i = threadIdx.x; i < rows; i += blockDim.x) m = fmaxf(m, fmaxf(fabsf(g[i]), gz ? fabsf(g[i] + gz[i]) : 0.f));
+  for (int i = threadIdx.x; i < rows; i += blockDim.x) m = fmaxf(m, fmaxf(fabsf(g[i]), gz ? fabsf(g[i] + 2.f * z_coef * logz[i] * gz[i]) : 0.f));
   m = block_max(m, scratch);
   const float u = (m > 1e-30f && m < 1e30f) ? m : 1.f;
   if (threadIdx.x == 0) *unit = u;
   for (int i = threadIdx.x; i < rows; i += blockDim.x) {
-    coef[i] = (gz ? g[i] + gz[i] : g[i]) / u;
+    coef[i] = (gz ? g[i] + 2.f * z_coef * logz[i] * gz[i] : g[i]) / u;
     gn[i] = g[i] / u;
   }
 }
@@ -152,13 +154,8 @@ PSched ce_whole_tiles(int M, int N, int K, bool& fits) {
 
 bool ce_operand_ok(const void* p, int64_t ld) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld % 64 == 0; }
 
-}  // namespace
-
-// part: fp32 pairs [ceil(V / 256)][T]; tgt: fp32 [T] (written where the target is in [vocab_start, vocab_start + V)).
-// x [T, H] and w [V, H] bf16, rows 16-byte aligned at pitches ldx, ldw (multiples of 64), H a multiple of 64.
-NTB_EXPORT int ntb_linear_ce_stats(const void* x, int64_t ldx, const void* w, int64_t ldw, const int64_t* target, int64_t vocab_start, int T, int V, int H, void* part,
-                                   float* tgt, int* status, int num_sms, cudaStream_t stream) {
-  if (T <= 0 || V <= 0 || H <= 0 || H % 64 || !ce_operand_ok(x, ldx) || !ce_operand_ok(w, ldw) || num_sms < 2 || !p_get_encode()) return NTB_ERR_ARG;
+int ce_stats(const void* x, int64_t ldx, const void* w, int64_t ldw, const int64_t* target, int64_t vocab_start, int T, int V, int H, void* part, float* tgt, int* status,
+             int num_sms, cudaStream_t stream) {
   bool fits;
   const PSched sched = ce_whole_tiles(T, V, H, fits);
   CUtensorMap ta, tb;
@@ -171,35 +168,13 @@ NTB_EXPORT int ntb_linear_ce_stats(const void* x, int64_t ldx, const void* w, in
   return ce_launch<false, false, P_OUT_CE_STATS>(ta, tb, ta, T, V, H, sched, ta, a, status, num_sms, stream);
 }
 
-// Joins the tiles of every token.  out_max / out_sum / out_tgt (all or none): the three numbers that vocabulary shards exchange;
-// logz / loss (both or none): the finished values where this is the whole vocabulary.
-NTB_EXPORT int ntb_linear_ce_join(const void* part, const float* tgt, const int64_t* target, int64_t vocab_start, int T, int V, float* out_max, float* out_sum,
-                                  float* out_tgt, float* logz, float* loss, cudaStream_t stream) {
-  if (T <= 0 || V <= 0 || (out_max != nullptr) != (out_sum != nullptr) || (out_max != nullptr) != (out_tgt != nullptr) || (logz != nullptr) != (loss != nullptr)) return NTB_ERR_ARG;
-  const int tiles = (V + P_BLOCK_N - 1) / P_BLOCK_N;
-  ce_join_kernel<<<(T + CE_JOIN_ROWS - 1) / CE_JOIN_ROWS, CE_JOIN_ROWS * CE_JOIN_PARTS, 0, stream>>>(static_cast<const float2*>(part), tgt, target, vocab_start, V, tiles, T, out_max,
-                                                                                                     out_sum, out_tgt, logz, loss);
-  return ntb_check_launch();
-}
-
-// g, gz (or null), coef, gn: fp32 [T]; unit: one fp32.
-NTB_EXPORT int ntb_linear_ce_row_coefficients(const float* g, const float* gz, int T, float* coef, float* gn, float* unit, cudaStream_t stream) {
-  if (T <= 0) return NTB_ERR_ARG;
-  ce_row_coefficients_kernel<<<1, 1024, 0, stream>>>(g, gz, T, coef, gn, unit);
-  return ntb_check_launch();
-}
-
-// d [T, V] bf16 at pitch ldd (a multiple of 64, at least V rounded up to 64; the columns up to there are written, as zeros), for the V
-// rows of w from vocabulary entry `vocab_start` on.
-NTB_EXPORT int ntb_linear_ce_dlogits(const void* x, int64_t ldx, const void* w, int64_t ldw, const int64_t* target, int64_t vocab_start, const float* logz,
-                                     const float* coef, const float* gn, int T, int V, int H, void* d, int64_t ldd, int* status, int num_sms, cudaStream_t stream) {
-  if (T <= 0 || V <= 0 || H <= 0 || H % 64 || !ce_operand_ok(x, ldx) || !ce_operand_ok(w, ldw) || !ce_operand_ok(d, ldd) || num_sms < 2 || !p_get_encode()) return NTB_ERR_ARG;
-  const int64_t width = (static_cast<int64_t>(V) + 63) / 64 * 64;
-  if (ldd < width) return NTB_ERR_ARG;
+// d [T, V] at pitch ldd; the columns up to V rounded up to 64 are written (zeros behind V).
+int ce_dlogits(const void* x, int64_t ldx, const void* w, int64_t ldw, const int64_t* target, int64_t vocab_start, const float* logz, const float* coef, const float* gn,
+               int T, int V, int H, void* d, int64_t ldd, int* status, int num_sms, cudaStream_t stream) {
   bool fits;
   const PSched sched = ce_whole_tiles(T, V, H, fits);
   CUtensorMap ta, tb, td;
-  if (!fits || !p_map_kmajor(&ta, x, T, H, ldx) || !p_map_kmajor(&tb, w, V, H, ldw) || !p_map_out(&td, d, T, width, ldd, false)) return NTB_ERR_ARG;
+  if (!fits || !p_map_kmajor(&ta, x, T, H, ldx) || !p_map_kmajor(&tb, w, V, H, ldw) || !p_map_out(&td, d, T, (static_cast<int64_t>(V) + 63) / 64 * 64, ldd, false)) return NTB_ERR_ARG;
   PCeArgs a;
   a.target = target;
   a.col0 = vocab_start;
@@ -209,31 +184,54 @@ NTB_EXPORT int ntb_linear_ce_dlogits(const void* x, int64_t ldx, const void* w, 
   return ce_launch<false, false, P_OUT_CE_GRAD>(ta, tb, td, T, V, H, sched, ta, a, status, num_sms, stream);
 }
 
-// How the dx product [T, H] over V is cut along V: with fewer tiles than CTA pairs (few tokens) every tile becomes `split` chunks
-// whose fp32 partial sums go through a workspace and are added in chunk order.  Returns the chunks per tile (1: not cut).
-NTB_EXPORT int ntb_linear_ce_dx_split(int T, int V, int H, int num_sms) {
-  const int pairs = num_sms / 2;
-  const int tiles = ((T + 255) / 256) * ((H + 255) / 256);
-  const int kb = (V + P_BLOCK_K - 1) / P_BLOCK_K;
-  if (tiles >= 2 * pairs) return 1;
-  // fewest rounds of (chunk length + a fixed share for the start and the hand-over of a chunk, about eight k-blocks)
-  int best = 1;
-  long long best_cost = -1;
-  for (int s = 1; s <= 64 && s * 8 <= kb + 7 && tiles * s <= 4 * pairs; s++) {
-    const long long rounds = (static_cast<long long>(tiles) * s + pairs - 1) / pairs;
-    const long long cost = rounds * ((kb + s - 1) / s + 8);
-    if (best_cost < 0 || cost < best_cost) best = s, best_cost = cost;
+// D tile = the sum, in chunk order, of the tile's workspace slabs (see PSched); bf16: scaled by *unit and rounded; fp32: stored, or added
+// with `accumulate`.  One thread per eight columns, one block per tile and 8 rows: a product cut for lack of tiles has few tiles, so
+// the sum takes its parallelism from the rows.
+__global__ void __launch_bounds__(256) ce_split_sum_kernel(const float* __restrict__ ws, void* __restrict__ out, int64_t ldo, int M, int N, int split, int chunks, int tiles_m,
+                                                            int tiles_n, int band, int bf16_out, int accumulate, const float* __restrict__ unit) {
+  const int tile = blockIdx.x >> 5;
+  const PTile tc = pair_tile(tile, tiles_m, tiles_n, band);
+  const int r = (blockIdx.x & 31) * 8 + (threadIdx.x >> 5), c8 = (threadIdx.x & 31) * 8;
+  const int row = tc.m_blk * 2 * P_BLOCK_M + r, col = tc.n_blk * P_BLOCK_N + c8;
+  if (row >= M || col >= N) return;
+  constexpr int64_t slab = static_cast<int64_t>(2 * P_BLOCK_M) * P_BLOCK_N;
+  const float* src = ws + static_cast<int64_t>(tile) * split * slab + r * P_BLOCK_N + c8;
+  float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int ch = 0; ch < chunks; ch++) {
+    Vec8<float> a;
+    float v[8];
+    a.load(src + ch * slab);
+    a.to_float(v);
+#pragma unroll
+    for (int j = 0; j < 8; j++) f[j] += v[j];
   }
-  return best;
+  if (bf16_out) {
+    const float u = *unit;
+#pragma unroll
+    for (int j = 0; j < 8; j++) f[j] *= u;
+    Vec8<__nv_bfloat16> o;
+    o.from_float(f);
+    o.store(static_cast<__nv_bfloat16*>(out) + static_cast<int64_t>(row) * ldo + col);
+  } else {
+    float* dst = static_cast<float*>(out) + static_cast<int64_t>(row) * ldo + col;
+    Vec8<float> o;
+    if (accumulate) {
+      float v[8];
+      o.load(dst);
+      o.to_float(v);
+#pragma unroll
+      for (int j = 0; j < 8; j++) f[j] += v[j];
+    }
+    o.from_float(f);
+    o.store(dst);
+  }
 }
 
-// dx (+)= d w over the V columns of d.  mode 0: dx bf16 = unit * sum; 1: dx fp32 = sum; 2: dx fp32 += sum (one launch at a time on a
-// buffer).  ws: fp32, split * tiles * 65536 elements when split > 1 (not needed otherwise).
-NTB_EXPORT int ntb_linear_ce_dx(const void* d, int64_t ldd, const void* w, int64_t ldw, void* dx, int64_t lddx, int T, int V, int H, int mode, const float* unit,
-                                int split, float* ws, int* status, int num_sms, cudaStream_t stream) {
-  if (T <= 0 || V <= 0 || H <= 0 || H % 64 || !ce_operand_ok(d, ldd) || !ce_operand_ok(w, ldw) || !ce_operand_ok(dx, lddx) || mode < 0 || mode > 2 || num_sms < 2 ||
-      split < 1 || (split > 1 && ws == nullptr) || (reinterpret_cast<uintptr_t>(ws) & 127) || !p_get_encode())
-    return NTB_ERR_ARG;
+// dx (+)= d w over the V columns of d.  mode 0: dx bf16 = unit * sum; 1: dx fp32 = sum; 2: dx fp32 += sum.  ws: fp32, split * tiles slabs
+// of 65536 when split > 1.
+int ce_dx(const void* d, int64_t ldd, const void* w, int64_t ldw, void* dx, int64_t lddx, int T, int V, int H, int mode, const float* unit, int split, float* ws,
+          int* status, int num_sms, cudaStream_t stream) {
   bool fits;
   PSched sched = ce_whole_tiles(T, H, V, fits);
   const int tiles = sched.total_units, kb = sched.kb_per;
@@ -254,28 +252,14 @@ NTB_EXPORT int ntb_linear_ce_dx(const void* d, int64_t ldd, const void* w, int64
   else if (mode == 1) rc = ce_launch<false, true, P_OUT_F32>(ta, tb, td, T, H, V, sched, tws, a, status, num_sms, stream);
   else rc = ce_launch<false, true, P_OUT_F32_ACCUM>(ta, tb, td, T, H, V, sched, tws, a, status, num_sms, stream);
   if (rc != NTB_OK || split == 1) return rc;
-  const int tiles_m = (T + 2 * P_BLOCK_M - 1) / (2 * P_BLOCK_M), tiles_n = (H + P_BLOCK_N - 1) / P_BLOCK_N, band = ce_band(T, V);
-  if (mode == 0) gemm2_split_fixup_kernel<P_OUT_BF16><<<tiles * 8, 256, 0, stream>>>(ws, dx, lddx, T, H, kb, sched, tiles_m, tiles_n, band, 0, unit);
-  else if (mode == 1) gemm2_split_fixup_kernel<P_OUT_F32><<<tiles * 8, 256, 0, stream>>>(ws, dx, lddx, T, H, kb, sched, tiles_m, tiles_n, band, 0);
-  else gemm2_split_fixup_kernel<P_OUT_F32_ACCUM><<<tiles * 8, 256, 0, stream>>>(ws, dx, lddx, T, H, kb, sched, tiles_m, tiles_n, band, 0);
-  return ntb_check_launch();
-}
-
-// out [n] bf16 = unit * acc [n] fp32; n a multiple of 8, both 16-byte aligned.
-NTB_EXPORT int ntb_linear_ce_scale_cast(const float* acc, const float* unit, void* out, int64_t n, cudaStream_t stream) {
-  if (n <= 0 || n % 8 || ((reinterpret_cast<uintptr_t>(acc) | reinterpret_cast<uintptr_t>(out)) & 15)) return NTB_ERR_ARG;
-  int64_t blocks = (n / 8 + 255) / 256;
-  if (blocks > 148 * 8) blocks = 148 * 8;
-  ce_scale_cast_kernel<<<static_cast<unsigned>(blocks), 256, 0, stream>>>(acc, unit, static_cast<__nv_bfloat16*>(out), n / 8);
+  const int chunks = (kb + sched.kb_per - 1) / sched.kb_per;  // chunks past the end of K wrote nothing
+  ce_split_sum_kernel<<<tiles * 32, 256, 0, stream>>>(ws, dx, lddx, T, H, split, chunks, (T + 255) / 256, (H + 255) / 256, ce_band(T, V), mode == 0, mode == 2, unit);
   return ntb_check_launch();
 }
 
 // Rows of the weight gradient: dw [V, H] = unit * d^T x (accumulate 0: bf16 store; 1: added to fp32 dw).
-NTB_EXPORT int ntb_linear_ce_dw(const void* d, int64_t ldd, const void* x, int64_t ldx, void* dw, int64_t lddw, int T, int V, int H, int accumulate, const float* unit,
-                                int* status, int num_sms, cudaStream_t stream) {
-  if (T <= 0 || V <= 0 || H <= 0 || H % 64 || !ce_operand_ok(d, ldd) || !ce_operand_ok(x, ldx) || (reinterpret_cast<uintptr_t>(dw) & 15) || lddw % 8 || num_sms < 2 ||
-      !p_get_encode())
-    return NTB_ERR_ARG;
+int ce_dw(const void* d, int64_t ldd, const void* x, int64_t ldx, void* dw, int64_t lddw, int T, int V, int H, int accumulate, const float* unit, int* status, int num_sms,
+          cudaStream_t stream) {
   bool fits;
   const PSched sched = ce_whole_tiles(V, H, T, fits);
   CUtensorMap ta, tb, td;
@@ -284,4 +268,80 @@ NTB_EXPORT int ntb_linear_ce_dw(const void* d, int64_t ldd, const void* x, int64
   a.alpha = unit;
   if (accumulate) return ce_launch<true, true, P_OUT_F32_ACCUM>(ta, tb, td, V, H, T, sched, ta, a, status, num_sms, stream);
   return ce_launch<true, true, P_OUT_BF16>(ta, tb, td, V, H, T, sched, ta, a, status, num_sms, stream);
+}
+
+}  // namespace
+
+// x [T, H] and w [V, H] bf16, rows 16-byte aligned at pitches ldx, ldw (multiples of 64), H a multiple of 64; target int64 [T]; this
+// rank's rows of the vocabulary start at vocab_start.  part: fp32 scratch, (ceil(V / 256) * 2 + 1) * T elements, 8-byte aligned.
+// out: fp32 planes of T: with finish, logZ, loss and (z_coef > 0) z_coef logZ^2; without, the three numbers that vocabulary shards
+// exchange: largest score, sum of exp(score - largest), the target's score or 0.
+NTB_EXPORT int ntb_linear_ce_forward(const void* x, int64_t ldx, const void* w, int64_t ldw, const int64_t* target, int64_t vocab_start, int T, int V, int H, float* part,
+                                     float* out, int finish, float z_coef, int* status, int num_sms, cudaStream_t stream) {
+  if (T <= 0 || V <= 0 || H <= 0 || H % 64 || !ce_operand_ok(x, ldx) || !ce_operand_ok(w, ldw) || (reinterpret_cast<uintptr_t>(part) & 7) || num_sms < 2 || !p_get_encode()) return NTB_ERR_ARG;
+  const int tiles = (V + P_BLOCK_N - 1) / P_BLOCK_N;
+  float* tgt = part + static_cast<int64_t>(tiles) * 2 * T;
+  const int rc = ce_stats(x, ldx, w, ldw, target, vocab_start, T, V, H, part, tgt, status, num_sms, stream);
+  if (rc != NTB_OK) return rc;
+  float *a = out, *b = out + T, *c = out + 2 * static_cast<int64_t>(T);
+  ce_join_kernel<<<(T + CE_JOIN_ROWS - 1) / CE_JOIN_ROWS, CE_JOIN_ROWS * CE_JOIN_PARTS, 0, stream>>>(
+      reinterpret_cast<const float2*>(part), tgt, target, vocab_start, V, tiles, T, finish ? nullptr : a, finish ? nullptr : b, finish ? nullptr : c, finish ? a : nullptr,
+      finish ? b : nullptr, finish && z_coef > 0.f ? c : nullptr, z_coef);
+  return ntb_check_launch();
+}
+
+// How the dx product [T, H] over V is cut along V: with fewer tiles than CTA pairs (few tokens) every tile becomes `split` chunks
+// whose fp32 partial sums go through a workspace and are added in chunk order.  Returns the chunks per tile (1: not cut).
+NTB_EXPORT int ntb_linear_ce_dx_split(int T, int V, int H, int num_sms) {
+  const int pairs = num_sms / 2;
+  const long long tiles = ((T + 255ll) / 256) * ((H + 255) / 256);
+  const int kb = (V + P_BLOCK_K - 1) / P_BLOCK_K;
+  if (tiles >= 2 * pairs) return 1;
+  // fewest rounds of (chunk length + a fixed share for the start and the hand-over of a chunk, about eight k-blocks)
+  int best = 1;
+  long long best_cost = -1;
+  for (int s = 1; s <= 64 && s * 8 <= kb + 7 && tiles * s <= 4 * pairs; s++) {
+    const long long rounds = (tiles * s + pairs - 1) / pairs;
+    const long long cost = rounds * ((kb + s - 1) / s + 8);
+    if (best_cost < 0 || cost < best_cost) best = s, best_cost = cost;
+  }
+  return best;
+}
+
+// Gradients, in pieces of `width` vocabulary entries.  g, gz (null without a z term), logz: fp32 [T].
+// d: bf16 [T, ldd], ldd a multiple of 64 and at least min(width, V); rows: fp32 scratch, 2 T + 1; acc: fp32 [T, H] when there are
+// several pieces and dx is wanted; ws: fp32, split * ceil(T / 256) * ceil(H / 256) * 65536 when split (ntb_linear_ce_dx_split of a
+// piece) > 1.  dx: bf16 [T, H] or null; dw: [V, H] at pitch lddw or null, bf16 (dw_accumulate 0) or fp32 that is added to (1).
+NTB_EXPORT int ntb_linear_ce_backward(const void* x, int64_t ldx, const void* w, int64_t ldw, const int64_t* target, int64_t vocab_start, const float* logz, const float* g,
+                                      const float* gz, float z_coef, int T, int V, int H, int width, void* d, int64_t ldd, float* rows, void* dx, float* acc, int split,
+                                      float* ws, void* dw, int64_t lddw, int dw_accumulate, int* status, int num_sms, cudaStream_t stream) {
+  if (T <= 0 || V <= 0 || H <= 0 || H % 64 || width <= 0 || width % 64 || !ce_operand_ok(x, ldx) || !ce_operand_ok(w, ldw) || !ce_operand_ok(d, ldd) || num_sms < 2 ||
+      ldd < (static_cast<int64_t>(width < V ? width : V) + 63) / 64 * 64 || !p_get_encode())
+    return NTB_ERR_ARG;
+  if (dx != nullptr && (!ce_operand_ok(dx, H) || (width < V && (acc == nullptr || !ce_operand_ok(acc, H))) || split < 1 || (split > 1 && (ws == nullptr || (reinterpret_cast<uintptr_t>(ws) & 127)))))
+    return NTB_ERR_ARG;
+  if (dw != nullptr && ((reinterpret_cast<uintptr_t>(dw) & 15) || lddw % 8 || lddw < H)) return NTB_ERR_ARG;
+  float *coef = rows, *gn = rows + T, *unit = rows + 2 * static_cast<int64_t>(T);
+  ce_row_coefficients_kernel<<<1, 1024, 0, stream>>>(g, gz, logz, z_coef, T, coef, gn, unit);
+  for (int64_t v0 = 0; v0 < V; v0 += width) {
+    const int n = static_cast<int>(V - v0 < width ? V - v0 : width);
+    const char* wp = static_cast<const char*>(w) + v0 * ldw * 2;
+    int rc = ce_dlogits(x, ldx, wp, ldw, target, vocab_start + v0, logz, coef, gn, T, n, H, d, ldd, status, num_sms, stream);
+    if (rc != NTB_OK) return rc;
+    if (dx != nullptr) {
+      rc = width >= V ? ce_dx(d, ldd, wp, ldw, dx, H, T, n, H, 0, unit, split, ws, status, num_sms, stream)
+                      : ce_dx(d, ldd, wp, ldw, acc, H, T, n, H, v0 == 0 ? 1 : 2, unit, split, ws, status, num_sms, stream);
+      if (rc != NTB_OK) return rc;
+    }
+    if (dw != nullptr) {
+      rc = ce_dw(d, ldd, x, ldx, static_cast<char*>(dw) + v0 * lddw * (dw_accumulate ? 4 : 2), lddw, T, n, H, dw_accumulate, unit, status, num_sms, stream);
+      if (rc != NTB_OK) return rc;
+    }
+  }
+  if (dx != nullptr && width < V) {
+    const int64_t n8 = static_cast<int64_t>(T) * H / 8;
+    const int64_t blocks = (n8 + 255) / 256;
+    ce_scale_cast_kernel<<<static_cast<unsigned>(blocks < 148 * 8 ? blocks : 148 * 8), 256, 0, stream>>>(acc, unit, static_cast<__nv_bfloat16*>(dx), n8);
+  }
+  return ntb_check_launch();
 }

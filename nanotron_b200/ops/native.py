@@ -10,6 +10,7 @@ from __future__ import annotations
 import ctypes
 import os
 import struct
+from array import array
 from ctypes import c_float, c_int, c_int64, c_void_p
 from pathlib import Path
 from typing import List, Optional, Tuple
@@ -51,7 +52,7 @@ def _declare(L):
     L.ntb_ce_backward.argtypes = [c_int] + [c_void_p] * 6 + [c_int64, c_int, c_int64, c_void_p]
     L.ntb_adamw_flat.argtypes = [c_void_p] * 5 + [c_int64] + [c_void_p] * 3 + [c_int] + [c_float] * 5 + [c_void_p, c_void_p]
     L.ntb_adamw_multi.restype = c_int
-    L.ntb_adamw_multi.argtypes = [c_void_p, c_int, c_int, c_int, c_int] + [c_float] * 7 + [c_void_p, c_int, c_void_p]
+    L.ntb_adamw_multi.argtypes = [c_void_p, c_int, c_int, c_int, c_int] + [c_float] * 7 + [c_void_p, ctypes.c_uint32, c_int, c_void_p]
     L.ntb_q8_decode.restype = c_int
     L.ntb_q8_decode.argtypes = [c_void_p, c_void_p, c_void_p, c_int64, c_int, c_int, c_void_p]
     L.ntb_q8_encode.restype = c_int
@@ -108,10 +109,30 @@ def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
     return None if t is None else t.data_ptr()
 
 
-def _check(rc: int, what: str):
+class on_device:
+    """``torch.cuda.device(dev)`` that costs one call where ``dev`` is the current device already (small operators are bound by the host)."""
+
+    __slots__ = ("index", "previous")
+
+    def __init__(self, dev: torch.device):
+        self.index, self.previous = dev.index, -1
+
+    def __enter__(self):
+        current = torch.cuda.current_device()
+        if self.index is not None and self.index != current:
+            self.previous = current
+            torch.cuda.set_device(self.index)
+
+    def __exit__(self, *exc):
+        if self.previous >= 0:
+            torch.cuda.set_device(self.previous)
+        return False
+
+
+def _check(rc: int, what: str, launches: int = 1):
     from nanotron_b200.ops import LAUNCH_COUNTER
 
-    LAUNCH_COUNTER["n"] += 1
+    LAUNCH_COUNTER["n"] += launches
     if rc != 0:
         detail = {1: "unsupported shape or alignment", 2: "CUDA launch error", 3: "device-side wait timed out"}.get(rc, "unknown")
         raise NativeKernelError(f"{what} failed with status {rc} ({detail})")
@@ -242,42 +263,44 @@ def adamw_flat(p, g, m, v, p16, seg_end, seg_lr, seg_wd, beta1, beta2, eps, step
     _check(rc, "adamw_flat")
 
 
-_AM_RECORD = struct.Struct("@7Qq2f2I")  # AmTensor of csrc/optim_multi.cu
+_AM_WORDS = struct.Struct("@2f")
 
 
 def adamw_multi(params, grads, exp_avgs, exp_avg_sqs, lrs, beta1, beta2, eps, weight_decays, step, halves, exp_avg_exponents, exp_avg_sq_exponents, grad_scale, seed):
     """One launch for all tensors (one per pair of parameter and gradient type, and per 384 tensors).  The addresses travel as kernel
-    parameters, so nothing is copied to the device."""
+    parameters, so nothing is copied to the device.  ``lrs``, ``weight_decays``: a number or one per tensor."""
     from nanotron_b200.ops import native_gemm
-    from nanotron_b200.ops.reference import q8_tensor_key
 
-    dev = params[0].device
+    dev, count = params[0].device, len(params)
     eight = exp_avg_exponents is not None
-    bc1, bc2 = 1.0 - beta1**step, 1.0 - beta2**step
-    records, kept = {}, []
-    for i, (p, g, m, v) in enumerate(zip(params, grads, exp_avgs, exp_avg_sqs)):
-        n = p.numel()
-        if n == 0:
-            continue
-        if not g.is_contiguous():
-            g = g.contiguous()
-            kept.append(g)
-        h = halves[i] if halves is not None else None
-        records.setdefault((p.dtype, g.dtype), []).append(
-            _AM_RECORD.pack(p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), 0 if h is None else h.data_ptr(), exp_avg_exponents[i].data_ptr() if eight else 0,
-                            exp_avg_sq_exponents[i].data_ptr() if eight else 0, n, lrs[i], weight_decays[i], q8_tensor_key(seed, i) if eight else 0, 0))
+    kept = [g if g.is_contiguous() else g.contiguous() for g in grads]
+    # records of AmTensor (csrc/optim_multi.cu) as ten 64-bit words: addresses, size, (lr, weight decay), (list position, 0)
+    none = (0,) * count
+    rates = [int.from_bytes(_AM_WORDS.pack(a, b), "little") for a, b in zip(lrs, weight_decays)] if isinstance(lrs, list) or isinstance(weight_decays, list) else None
+    if rates is None:
+        rates = (int.from_bytes(_AM_WORDS.pack(lrs, weight_decays), "little"),) * count
+    rows = list(zip(
+        [t.data_ptr() for t in params], [t.data_ptr() for t in kept], [t.data_ptr() for t in exp_avgs], [t.data_ptr() for t in exp_avg_sqs],
+        [0 if t is None else t.data_ptr() for t in halves] if halves is not None else none,
+        [t.data_ptr() for t in exp_avg_exponents] if eight else none, [t.data_ptr() for t in exp_avg_sq_exponents] if eight else none,
+        [t.numel() for t in params], rates, range(count),
+    ))
+    kinds = [(p.dtype, g.dtype) for p, g in zip(params, kept)]
     L = lib()
-    with torch.cuda.device(dev):
-        for (pt, gt), rows in records.items():
-            table = ctypes.create_string_buffer(b"".join(rows), len(rows) * _AM_RECORD.size)
-            _check(L.ntb_adamw_multi(table, len(rows), _DT[pt], _DT[gt], 8 if eight else 32, beta1, 1.0 - beta1, beta2, 1.0 - beta2, eps, bc1, bc2, _ptr(grad_scale),
-                                     native_gemm._sms(dev), _stream(params[0])), "adamw_multi")
+    with on_device(dev):
+        for kind in set(kinds):
+            words = array("Q", [w for row, k in zip(rows, kinds) if k == kind and row[7] for w in row])
+            if not words:
+                continue
+            _check(L.ntb_adamw_multi(words.buffer_info()[0], len(words) // 10, _DT[kind[0]], _DT[kind[1]], 8 if eight else 32, beta1, 1.0 - beta1, beta2, 1.0 - beta2, eps,
+                                     1.0 - beta1**step, 1.0 - beta2**step, _ptr(grad_scale), seed & 0xFFFFFFFF, native_gemm._sms(dev), _stream(params[0])),
+                   "adamw_multi", launches=(len(words) // 10 + 383) // 384)
 
 
 def q8_decode(codes, exponents, signed: bool, dtype):
     out = torch.empty(codes.shape, dtype=dtype, device=codes.device)
     if codes.numel():
-        with torch.cuda.device(codes.device):
+        with on_device(codes.device):
             _check(lib().ntb_q8_decode(codes.data_ptr(), exponents.data_ptr(), out.data_ptr(), codes.numel(), int(signed), _DT[dtype], _stream(codes)), "q8_decode")
     return out
 
@@ -286,7 +309,7 @@ def q8_encode(x, signed: bool):
     codes = torch.empty(x.shape, dtype=torch.uint8, device=x.device)
     exponents = torch.empty((x.numel() + 127) // 128, dtype=torch.uint8, device=x.device)
     if x.numel():
-        with torch.cuda.device(x.device):
+        with on_device(x.device):
             _check(lib().ntb_q8_encode(x.data_ptr(), codes.data_ptr(), exponents.data_ptr(), x.numel(), int(signed), _stream(x)), "q8_encode")
     return codes, exponents
 

@@ -182,13 +182,15 @@ def linear_ce_partials(x, weight, target, vocab_start: int, piece: int = 8192):
     return m, s, t
 
 
-def linear_ce_backward(x, weight, target, logz, grad_loss, grad_z, vocab_start: int, piece: int = 8192):
-    """Gradients (of ``x`` and ``weight``, in their types) of the losses whose log-partition is ``logz``, by pieces of the vocabulary."""
+def linear_ce_backward(x, weight, target, logz, grad_loss, grad_z, z_coef: float, vocab_start: int, piece: int = 8192):
+    """Gradients (of ``x`` and ``weight``, in their types) of the losses whose log-partition is ``logz`` and of the terms z_coef logz^2, by
+    pieces of the vocabulary."""
     xf = _wide(x)
+    coef = grad_loss if grad_z is None else grad_loss + 2.0 * z_coef * logz * grad_z
     dx, dw = torch.zeros_like(xf), torch.empty(weight.shape, dtype=xf.dtype, device=x.device)
     for a in range(0, weight.shape[0], piece):
         wp = _wide(weight[a : a + piece])
-        d = torch.exp(xf @ wp.t() - logz.unsqueeze(-1)) * (grad_loss if grad_z is None else grad_loss + grad_z).unsqueeze(-1)
+        d = torch.exp(xf @ wp.t() - logz.unsqueeze(-1)) * coef.unsqueeze(-1)
         local = target - vocab_start - a
         sub = torch.where((local >= 0) & (local < wp.shape[0]), grad_loss, torch.zeros_like(grad_loss))
         d.scatter_add_(-1, local.clamp(0, wp.shape[0] - 1).unsqueeze(-1), -sub.unsqueeze(-1).to(d.dtype))
@@ -312,6 +314,8 @@ def q8_decode(codes: torch.Tensor, exponents: torch.Tensor, signed: bool, dtype:
 def adamw_multi_tensor(params, grads, exp_avgs, exp_avg_sqs, lrs, beta1, beta2, eps, weight_decays, step, halves, exp_avg_exponents, exp_avg_sq_exponents, grad_scale, seed):
     """One AdamW step over lists of tensors, in place (see ``ops.adamw_multi_tensor``).  Every operation is rounded to fp32 by itself."""
     bc1, bc2 = 1 - beta1**step, 1 - beta2**step
+    lrs = lrs if isinstance(lrs, list) else [lrs] * len(params)
+    weight_decays = weight_decays if isinstance(weight_decays, list) else [weight_decays] * len(params)
     for i, (p, g, ms, vs) in enumerate(zip(params, grads, exp_avgs, exp_avg_sqs)):
         if p.numel() == 0:
             continue

@@ -294,10 +294,11 @@ class _LinearCrossEntropy(torch.autograd.Function):
         lead = x.shape[:-1]
         x2, tgt = x.reshape(-1, x.shape[-1]), target.reshape(-1).to(torch.int64).contiguous()
         vocab_start = rank * weight.shape[0]
+        z = None
         if x2.shape[0] == 0:
             logz = loss = torch.zeros(0, dtype=torch.float32, device=x.device)
         elif tp == 1:
-            logz, loss = ops.linear_ce_forward(x2, weight, tgt, 0, finish=True)
+            logz, loss, z = ops.linear_ce_forward(x2, weight, tgt, 0, finish=True, z_coef=z_loss_coef)
         else:
             local_max, local_sumexp, local_tgt = ops.linear_ce_forward(x2, weight, tgt, vocab_start, finish=False)
             fused = ops.tp_fused.get_context(group) if x.is_cuda and ops.tp_fused.ENABLED else None
@@ -310,9 +311,11 @@ class _LinearCrossEntropy(torch.autograd.Function):
                 dist.all_reduce(packed, op=dist.ReduceOp.SUM, group=group)
                 logz = gmax + torch.log(packed[0])
                 loss = logz - packed[1]
+        if z is None and z_loss_coef > 0:
+            z = z_loss_coef * logz.square()
         ctx.save_for_backward(x2, weight, tgt, logz)
         ctx.vocab_start, ctx.shape, ctx.z = vocab_start, x.shape, z_loss_coef
-        return loss.view(lead), ((z_loss_coef * logz.square()).view(lead) if z_loss_coef > 0 else None)
+        return loss.view(lead), (z.view(lead) if z is not None else None)
 
     @staticmethod
     @once_differentiable
@@ -323,8 +326,8 @@ class _LinearCrossEntropy(torch.autograd.Function):
             return (x2.new_zeros(ctx.shape) if need_dx else None), (torch.zeros_like(weight) if need_dw else None), None, None, None
         wide = logz.dtype
         g = grad_loss.reshape(-1).to(wide).contiguous()
-        gz = 2.0 * ctx.z * logz * grad_z.reshape(-1).to(wide) if ctx.z > 0 else None
-        dx, dw = ops.linear_ce_backward(x2, weight, tgt, logz, g, gz, ctx.vocab_start, need_dx, need_dw)
+        gz = grad_z.reshape(-1).to(wide).contiguous() if ctx.z > 0 else None
+        dx, dw = ops.linear_ce_backward(x2, weight, tgt, logz, g, gz, ctx.z, ctx.vocab_start, need_dx, need_dw)
         return (dx.view(ctx.shape) if need_dx else None), dw, None, None, None
 
 

@@ -46,7 +46,7 @@ def test_reference_pieces_match_the_definition(T, H, V, piece):
     m, s, t = ref.linear_ce_partials(x, w, y, 0, piece=piece)
     logz = m + s.log()
     torch.testing.assert_close(logz - t, loss, rtol=1e-12, atol=1e-12)
-    dx2, dw2 = ref.linear_ce_backward(x, w, y, logz, g, None, 0, piece=piece)
+    dx2, dw2 = ref.linear_ce_backward(x, w, y, logz, g, None, 0.0, 0, piece=piece)
     torch.testing.assert_close(dx2, dx, rtol=1e-12, atol=1e-12)
     torch.testing.assert_close(dw2, dw, rtol=1e-12, atol=1e-12)
 
