@@ -92,8 +92,6 @@ def native_launches() -> int:
 def _use_native(t: torch.Tensor) -> bool:
     if _MODE == "torch" or not t.is_cuda:
         return False
-    from nanotron_b200.ops import native
-
     native.lib()  # raises when the extension is missing: no silent fallback on GPU
     return True
 
@@ -389,8 +387,6 @@ def linear_ce_forward(x2: torch.Tensor, weight: torch.Tensor, target: torch.Tens
     whole vocabulary): (logZ, loss, z_coef logZ^2 or None) per token; otherwise the shard's (max, sum exp, target score or 0) like
     ``ce_partials``."""
     if _use_native(x2):
-        from nanotron_b200.ops import native_ce
-
         native_ce.check_operands(x2, weight, target)
         out = native_ce.forward(x2, weight, target, vocab_start, finish, z_coef).unbind(0)
         return out if len(out) == 3 else (*out, None)
@@ -406,8 +402,6 @@ def linear_ce_backward(x2, weight, target, logz, grad_loss, grad_z, z_coef: floa
     ``main_grad`` gets its gradient added there, and None is returned for it."""
     main_grad = getattr(weight, "main_grad", None) if need_dw else None
     if _use_native(x2):
-        from nanotron_b200.ops import native_ce
-
         direct = main_grad is not None and main_grad.dtype == torch.float32 and main_grad.stride(1) == 1 and main_grad.stride(0) % 8 == 0 and main_grad.data_ptr() % 16 == 0
         dx, dw = native_ce.backward(x2, weight, target, logz, grad_loss, grad_z, z_coef, vocab_start, need_dx, need_dw, main_grad if direct else None)
         if direct:
@@ -671,8 +665,6 @@ def q8_decode(codes: torch.Tensor, exponents: torch.Tensor, signed: bool, dtype:
     if dtype not in (torch.float32, torch.bfloat16):
         raise ValueError(f"q8_decode gives float32 or bfloat16, not {dtype}")
     if _use_native(codes):
-        from nanotron_b200.ops import native
-
         return native.q8_decode(codes, exponents, signed, dtype)
     return ref.q8_decode(codes, exponents, signed, dtype)
 
@@ -682,8 +674,6 @@ def q8_encode(x: torch.Tensor, signed: bool):
     if x.dtype != torch.float32:
         raise ValueError(f"q8_encode takes float32, got {x.dtype}")
     if _use_native(x):
-        from nanotron_b200.ops import native
-
         return native.q8_encode(x.contiguous(), signed)
     return ref.q8_encode(x, signed)
 
@@ -695,7 +685,6 @@ def _check_q8(codes, exponents, what):
                          f"{tuple(exponents.shape)} {exponents.dtype} on {exponents.device}")
 
 
-@torch.no_grad()
 def adamw_multi_tensor(params, grads, exp_avgs, exp_avg_sqs, *, lr, beta1: float, beta2: float, eps: float, weight_decay, step: float, halves=None,
                        exp_avg_exponents=None, exp_avg_sq_exponents=None, grad_scale: Optional[torch.Tensor] = None, seed: int = 0) -> None:
     """One AdamW step (decoupled decay, bias correction; ``torch.optim.AdamW``) over lists of tensors on one device, in place, in one
@@ -731,15 +720,50 @@ def adamw_multi_tensor(params, grads, exp_avgs, exp_avg_sqs, *, lr, beta1: float
     dev = params[0].device
     if grad_scale is not None and (grad_scale.dtype != torch.float32 or grad_scale.numel() != 1 or grad_scale.device != dev):
         raise ValueError("adamw_multi_tensor: grad_scale is one float32 on the parameters' device")
-    # whole lists at a time: for many small tensors these checks are a good part of the call
-    state_type, floats, sizes = (torch.uint8 if eight else torch.float32), {torch.float32, torch.bfloat16}, [p.numel() for p in params]
+    native_call = _use_native(params[0])
+    if native_call:
+        # whole lists against whole lists: with many small tensors the checks are a good part of the call
+        kinds = [(p.dtype, g.dtype) for p, g in zip(params, grads)]
+        sizes = [p.numel() for p in params]
+        pointers = [p.data_ptr() for p in params]
+        index = params[0].get_device()
+        facts = lambda tensors: [(t.dtype, t.numel(), t.get_device(), t.is_contiguous()) for t in tensors]  # noqa: E731
+        want = [(torch.uint8 if eight else torch.float32, n_, index, True) for n_ in sizes]
+        fine = (
+            facts(exp_avgs) == want and facts(exp_avg_sqs) == want and set(kinds) <= _ADAMW_KINDS and [g.numel() for g in grads] == sizes
+            and {p.get_device() for p in params} == {g.get_device() for g in grads} == {index} and all([p.is_contiguous() for p in params])
+            and (len(set(pointers)) == n or 0 in sizes)
+        )
+        if fine and eight:
+            want = [(torch.uint8, (n_ + 127) // 128, index, True) for n_ in sizes]
+            fine = facts(exp_avg_exponents) == want and facts(exp_avg_sq_exponents) == want
+    written = [h for h in halves if h is not None] if halves is not None else []
+    if native_call and written:
+        fine = fine and facts(written) == [(torch.bfloat16, n_, index, True) for n_, h in zip(sizes, halves) if h is not None]
+    if not native_call or not fine or 0 in sizes:
+        _check_adamw_lists(params, grads, exp_avgs, exp_avg_sqs, halves, written, exp_avg_exponents, exp_avg_sq_exponents)
+    if native_call:
+        native.adamw_multi(params, grads, exp_avgs, exp_avg_sqs, lr, beta1, beta2, eps, weight_decay, step, halves, exp_avg_exponents, exp_avg_sq_exponents, grad_scale, seed, kinds, sizes, pointers)
+        torch.autograd.graph.increment_version([*params, *exp_avgs, *exp_avg_sqs, *written])
+    else:
+        with torch.no_grad():
+            ref.adamw_multi_tensor(params, grads, exp_avgs, exp_avg_sqs, lr, beta1, beta2, eps, weight_decay, step, halves, exp_avg_exponents, exp_avg_sq_exponents, grad_scale, seed)
+
+
+_ADAMW_KINDS = {(p, g) for p in (torch.float32, torch.bfloat16) for g in (torch.float32, torch.bfloat16)}
+
+
+def _check_adamw_lists(params, grads, exp_avgs, exp_avg_sqs, halves, written, exp_avg_exponents, exp_avg_sq_exponents):
+    """Says what is wrong with the lists of ``adamw_multi_tensor``, if anything is."""
+    dev, sizes, floats = params[0].device, [p.numel() for p in params], {torch.float32, torch.bfloat16}
+    state_type = torch.float32 if exp_avg_exponents is None else torch.uint8
 
     def check(what, tensors, types, numels, contiguous=True):
         if not {t.dtype for t in tensors} <= types:
             raise ValueError(f"adamw_multi_tensor: {what} in {sorted(map(str, types))} expected, got {sorted({str(t.dtype) for t in tensors})}")
         if [t.numel() for t in tensors] != numels:
             raise ValueError(f"adamw_multi_tensor: {what}: the sizes {[t.numel() for t in tensors]} do not fit, {numels} expected")
-        if {t.device for t in tensors} != {dev}:
+        if any(t.device != dev for t in tensors):
             raise ValueError(f"adamw_multi_tensor: {what}: everything has to be on {dev}")
         if contiguous and not all([t.is_contiguous() for t in tensors]):
             raise ValueError(f"adamw_multi_tensor: {what} have to be contiguous")
@@ -748,24 +772,14 @@ def adamw_multi_tensor(params, grads, exp_avgs, exp_avg_sqs, *, lr, beta1: float
     check("gradients", grads, floats, sizes, contiguous=False)
     check("first moments", exp_avgs, {state_type}, sizes)
     check("second moments", exp_avg_sqs, {state_type}, sizes)
-    if eight:
+    if exp_avg_exponents is not None:
         blocks = [(k + 127) // 128 for k in sizes]
         check("first moments' exponents", exp_avg_exponents, {torch.uint8}, blocks)
         check("second moments' exponents", exp_avg_sq_exponents, {torch.uint8}, blocks)
-    written = [h for h in halves if h is not None] if halves is not None else []
-    if written:
-        check("halves", written, {torch.bfloat16}, [k for k, h in zip(sizes, halves) if h is not None])
+    check("halves", written, {torch.bfloat16}, [k for k, h in zip(sizes, halves or ()) if h is not None])
     addresses = [p.data_ptr() for p, k in zip(params, sizes) if k]
     if len(set(addresses)) != len(addresses):
         raise ValueError("adamw_multi_tensor: the same parameter twice")
-    args = (params, grads, exp_avgs, exp_avg_sqs, lr, beta1, beta2, eps, weight_decay, step, halves, exp_avg_exponents, exp_avg_sq_exponents, grad_scale, seed)
-    if _use_native(params[0]):
-        from nanotron_b200.ops import native
-
-        native.adamw_multi(*args)
-        torch.autograd.graph.increment_version([*params, *exp_avgs, *exp_avg_sqs, *written])
-    else:
-        ref.adamw_multi_tensor(*args)
 
 
-from nanotron_b200.ops import tp_fused  # noqa: E402,F401
+from nanotron_b200.ops import native, native_ce, tp_fused  # noqa: E402,F401

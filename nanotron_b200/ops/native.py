@@ -12,10 +12,13 @@ import os
 import struct
 from array import array
 from ctypes import c_float, c_int, c_int64, c_void_p
+from itertools import chain
 from pathlib import Path
 from typing import List, Optional, Tuple
 
 import torch
+
+from nanotron_b200 import ops
 
 _LIB = None
 _LIB_PATH = Path(__file__).resolve().parent / "libntb_kernels.so"
@@ -105,6 +108,11 @@ def _stream(t: torch.Tensor) -> int:
     return torch.cuda.current_stream(t.device).cuda_stream
 
 
+def raw_stream(t: torch.Tensor) -> int:
+    """``_stream`` without building a Stream object (2 us a call)."""
+    return torch._C._cuda_getCurrentRawStream(t.get_device())
+
+
 def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
     return None if t is None else t.data_ptr()
 
@@ -118,7 +126,7 @@ class on_device:
         self.index, self.previous = dev.index, -1
 
     def __enter__(self):
-        current = torch.cuda.current_device()
+        current = torch._C._cuda_getDevice()
         if self.index is not None and self.index != current:
             self.previous = current
             torch.cuda.set_device(self.index)
@@ -130,9 +138,7 @@ class on_device:
 
 
 def _check(rc: int, what: str, launches: int = 1):
-    from nanotron_b200.ops import LAUNCH_COUNTER
-
-    LAUNCH_COUNTER["n"] += launches
+    ops.LAUNCH_COUNTER["n"] += launches
     if rc != 0:
         detail = {1: "unsupported shape or alignment", 2: "CUDA launch error", 3: "device-side wait timed out"}.get(rc, "unknown")
         raise NativeKernelError(f"{what} failed with status {rc} ({detail})")
@@ -263,45 +269,43 @@ def adamw_flat(p, g, m, v, p16, seg_end, seg_lr, seg_wd, beta1, beta2, eps, step
     _check(rc, "adamw_flat")
 
 
-_AM_WORDS = struct.Struct("@2f")
+_AM_RATES = struct.Struct("@2f")
 
 
-def adamw_multi(params, grads, exp_avgs, exp_avg_sqs, lrs, beta1, beta2, eps, weight_decays, step, halves, exp_avg_exponents, exp_avg_sq_exponents, grad_scale, seed):
+def adamw_multi(params, grads, exp_avgs, exp_avg_sqs, lr, beta1, beta2, eps, weight_decay, step, halves, exp_avg_exponents, exp_avg_sq_exponents, grad_scale, seed, kinds, sizes, pointers):
     """One launch for all tensors (one per pair of parameter and gradient type, and per 384 tensors).  The addresses travel as kernel
-    parameters, so nothing is copied to the device.  ``lrs``, ``weight_decays``: a number or one per tensor."""
-    from nanotron_b200.ops import native_gemm
-
-    dev, count = params[0].device, len(params)
-    eight = exp_avg_exponents is not None
+    parameters, so nothing is copied to the device.  ``lr``, ``weight_decay``: a number for all, or lists; ``kinds``, ``sizes``, ``pointers``:
+    the (parameter, gradient) types, elements and addresses of the parameters."""
+    count, eight = len(params), exp_avg_exponents is not None
     kept = [g if g.is_contiguous() else g.contiguous() for g in grads]
     # records of AmTensor (csrc/optim_multi.cu) as ten 64-bit words: addresses, size, (lr, weight decay), (list position, 0)
     none = (0,) * count
-    rates = [int.from_bytes(_AM_WORDS.pack(a, b), "little") for a, b in zip(lrs, weight_decays)] if isinstance(lrs, list) or isinstance(weight_decays, list) else None
-    if rates is None:
-        rates = (int.from_bytes(_AM_WORDS.pack(lrs, weight_decays), "little"),) * count
-    rows = list(zip(
-        [t.data_ptr() for t in params], [t.data_ptr() for t in kept], [t.data_ptr() for t in exp_avgs], [t.data_ptr() for t in exp_avg_sqs],
+    rates = [int.from_bytes(_AM_RATES.pack(a, b), "little") for a, b in zip(lr, weight_decay)] if isinstance(lr, list) else (int.from_bytes(_AM_RATES.pack(lr, weight_decay), "little"),) * count
+    rows = zip(
+        pointers, [t.data_ptr() for t in kept], [t.data_ptr() for t in exp_avgs], [t.data_ptr() for t in exp_avg_sqs],
         [0 if t is None else t.data_ptr() for t in halves] if halves is not None else none,
         [t.data_ptr() for t in exp_avg_exponents] if eight else none, [t.data_ptr() for t in exp_avg_sq_exponents] if eight else none,
-        [t.numel() for t in params], rates, range(count),
-    ))
-    kinds = [(p.dtype, g.dtype) for p, g in zip(params, kept)]
-    L = lib()
-    with on_device(dev):
+        sizes, rates, range(count),
+    )
+    L, p0 = lib(), params[0]
+    alike = len(set(kinds)) == 1 and 0 not in sizes
+    rows = None if alike and (words := array("Q", chain.from_iterable(rows))) else list(rows)
+    with on_device(p0.device):
         for kind in set(kinds):
-            words = array("Q", [w for row, k in zip(rows, kinds) if k == kind and row[7] for w in row])
+            if not alike:
+                words = array("Q", [w for row, k in zip(rows, kinds) if k == kind and row[7] for w in row])
             if not words:
                 continue
-            _check(L.ntb_adamw_multi(words.buffer_info()[0], len(words) // 10, _DT[kind[0]], _DT[kind[1]], 8 if eight else 32, beta1, 1.0 - beta1, beta2, 1.0 - beta2, eps,
-                                     1.0 - beta1**step, 1.0 - beta2**step, _ptr(grad_scale), seed & 0xFFFFFFFF, native_gemm._sms(dev), _stream(params[0])),
-                   "adamw_multi", launches=(len(words) // 10 + 383) // 384)
+            rc = L.ntb_adamw_multi(words.buffer_info()[0], len(words) // 10, _DT[kind[0]], _DT[kind[1]], 8 if eight else 32, beta1, 1.0 - beta1, beta2, 1.0 - beta2, eps,
+                                   1.0 - beta1**step, 1.0 - beta2**step, _ptr(grad_scale), seed & 0xFFFFFFFF, native_gemm._sms(p0.device), raw_stream(p0))
+            _check(rc, "adamw_multi", launches=(len(words) // 10 + 383) // 384)
 
 
 def q8_decode(codes, exponents, signed: bool, dtype):
     out = torch.empty(codes.shape, dtype=dtype, device=codes.device)
     if codes.numel():
         with on_device(codes.device):
-            _check(lib().ntb_q8_decode(codes.data_ptr(), exponents.data_ptr(), out.data_ptr(), codes.numel(), int(signed), _DT[dtype], _stream(codes)), "q8_decode")
+            _check(lib().ntb_q8_decode(codes.data_ptr(), exponents.data_ptr(), out.data_ptr(), codes.numel(), int(signed), _DT[dtype], raw_stream(codes)), "q8_decode")
     return out
 
 
@@ -427,5 +431,6 @@ def gemm_fp8_blockscaled(a, b, out: Optional[torch.Tensor] = None, accumulate_fp
 
 
 # ---------------------------------------------------------------------------- GEMM / attention: see native_gemm / native_attn
+from nanotron_b200.ops import native_gemm  # noqa: E402
 from nanotron_b200.ops.native_attn import flash_attn_bwd, flash_attn_fwd, flash_attn_supported  # noqa: E402,F401
 from nanotron_b200.ops.native_gemm import gemm_nn, gemm_nt, gemm_supported, gemm_tn, gemm_tn_accum_fp32  # noqa: E402,F401

@@ -10,6 +10,8 @@ from typing import Optional
 
 import torch
 
+from nanotron_b200.ops import native, native_gemm
+
 PIECE_ELEMENTS = 1 << 27  # scores of one piece of the backward pass: 256 MiB of bf16
 PIECE_MIN = 4096          # narrowest piece: below it the sums of dx over the pieces cost more than the pieces save
 
@@ -45,8 +47,6 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
 
 
 def _status(device) -> torch.Tensor:
-    from nanotron_b200.ops import native, native_gemm
-
     if str(device) not in native_gemm._STATUS and torch.cuda.is_current_stream_capturing():
         raise native.NativeKernelError("the first tensor-core call on a device cannot be captured into a CUDA graph: run it once before the capture")
     return native_gemm.status_word(device)
@@ -55,8 +55,6 @@ def _status(device) -> torch.Tensor:
 def forward(x2: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, vocab_start: int, finish: bool, z_coef: float = 0.0) -> torch.Tensor:
     """fp32 planes [.., T]; ``finish``: logZ and loss of a whole vocabulary, and z_coef logZ^2 when that is positive; otherwise this
     shard's largest score, sum of exp(score - largest), and target score or 0."""
-    from nanotron_b200.ops import native, native_gemm
-
     x2, weight = _rows(x2), _rows(weight)
     (T, H), V, dev = x2.shape, weight.shape[0], x2.device
     with native.on_device(dev):
@@ -64,7 +62,7 @@ def forward(x2: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, vocab_
         part = torch.empty(((V + 255) // 256 * 2 + 1) * T, dtype=torch.float32, device=dev)  # per tile two numbers, and the target's score
         out = torch.empty((3 if z_coef > 0 or not finish else 2, T), dtype=torch.float32, device=dev)
         native._check(native.lib().ntb_linear_ce_forward(x2.data_ptr(), x2.stride(0), weight.data_ptr(), weight.stride(0), target.data_ptr(), vocab_start, T, V, H, part.data_ptr(),
-                                                         out.data_ptr(), int(finish), z_coef, status.data_ptr(), native_gemm._sms(dev), native._stream(x2)), "linear_ce_forward", launches=2)
+                                                         out.data_ptr(), int(finish), z_coef, status.data_ptr(), native_gemm._sms(dev), native.raw_stream(x2)), "linear_ce_forward", launches=2)
     return out
 
 
@@ -78,8 +76,6 @@ def piece_width(T: int, V: int) -> int:
 def backward(x2, weight, target, logz, g, gz: Optional[torch.Tensor], z_coef: float, vocab_start: int, need_dx: bool, need_dw: bool, main_grad: Optional[torch.Tensor] = None):
     """(dx, dw) in bf16 for the upstream gradients ``g`` of the losses and ``gz`` of the terms z_coef logZ^2 (fp32 [T]); with
     ``main_grad`` (fp32 [V, H]) dw is added to it and None is returned in its place."""
-    from nanotron_b200.ops import native, native_gemm
-
     x2, weight = _rows(x2), _rows(weight)
     (T, H), V, dev = x2.shape, weight.shape[0], x2.device
     L, sms, ptr = native.lib(), native_gemm._sms(dev), native._ptr
@@ -97,6 +93,6 @@ def backward(x2, weight, target, logz, g, gz: Optional[torch.Tensor], z_coef: fl
         pieces = (V + width - 1) // width
         rc = L.ntb_linear_ce_backward(x2.data_ptr(), x2.stride(0), weight.data_ptr(), weight.stride(0), target.data_ptr(), vocab_start, logz.data_ptr(), g.data_ptr(), ptr(gz), z_coef,
                                       T, V, H, width, d.data_ptr(), pitch, rows.data_ptr(), ptr(dx), ptr(acc), split, ptr(ws), ptr(into), into.stride(0) if need_dw else H,
-                                      int(main_grad is not None), _status(dev).data_ptr(), sms, native._stream(x2))
+                                      int(main_grad is not None), _status(dev).data_ptr(), sms, native.raw_stream(x2))
         native._check(rc, "linear_ce_backward", launches=1 + pieces * (1 + (1 + (split > 1)) * need_dx + need_dw) + (acc is not None))
     return dx, dw

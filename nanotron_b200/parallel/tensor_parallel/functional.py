@@ -282,6 +282,34 @@ def sharded_cross_entropy_with_z_loss(sharded_logits, target, group, dtype=None,
 
 
 # ----------------------------------------------------------------------------- cross entropy of a vocabulary-sharded linear head
+def _linear_cross_entropy_forward(x, weight, target, group, z_loss_coef: float):
+    tp = group.size() if group is not None else 1
+    rank = dist.get_rank(group) if tp > 1 else 0
+    lead = x.shape[:-1]
+    x2, tgt = x.reshape(-1, x.shape[-1]), target.reshape(-1).to(torch.int64).contiguous()
+    vocab_start = rank * weight.shape[0]
+    z = None
+    if x2.shape[0] == 0:
+        logz = loss = torch.zeros(0, dtype=torch.float32, device=x.device)
+    elif tp == 1:
+        logz, loss, z = ops.linear_ce_forward(x2, weight, tgt, 0, finish=True, z_coef=z_loss_coef)
+    else:
+        local_max, local_sumexp, local_tgt = ops.linear_ce_forward(x2, weight, tgt, vocab_start, finish=False)
+        fused = ops.tp_fused.get_context(group) if x.is_cuda and ops.tp_fused.ENABLED else None
+        if fused is not None:
+            logz, loss = fused.ce_combine(local_max, local_sumexp, local_tgt)  # tp reduction by peer loads inside the kernel
+        else:
+            gmax = local_max.clone()
+            dist.all_reduce(gmax, op=dist.ReduceOp.MAX, group=group)
+            packed = torch.stack([local_sumexp * torch.exp(local_max - gmax), local_tgt])
+            dist.all_reduce(packed, op=dist.ReduceOp.SUM, group=group)
+            logz = gmax + torch.log(packed[0])
+            loss = logz - packed[1]
+    if z is None and z_loss_coef > 0:
+        z = z_loss_coef * logz.square()
+    return loss.view(lead), (z.view(lead) if z is not None else None), x2, tgt, logz, vocab_start
+
+
 class _LinearCrossEntropy(torch.autograd.Function):
     """The head product and ``_ShardedCrossEntropy`` in one: the scores exist only on chip (forward) or one piece of the vocabulary at
     a time (backward, which computes them again), so no tensor of tokens x vocabulary is kept between the two.  Saved for backward:
@@ -289,33 +317,10 @@ class _LinearCrossEntropy(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, target, group, z_loss_coef: float):
-        tp = group.size() if group is not None else 1
-        rank = dist.get_rank(group) if tp > 1 else 0
-        lead = x.shape[:-1]
-        x2, tgt = x.reshape(-1, x.shape[-1]), target.reshape(-1).to(torch.int64).contiguous()
-        vocab_start = rank * weight.shape[0]
-        z = None
-        if x2.shape[0] == 0:
-            logz = loss = torch.zeros(0, dtype=torch.float32, device=x.device)
-        elif tp == 1:
-            logz, loss, z = ops.linear_ce_forward(x2, weight, tgt, 0, finish=True, z_coef=z_loss_coef)
-        else:
-            local_max, local_sumexp, local_tgt = ops.linear_ce_forward(x2, weight, tgt, vocab_start, finish=False)
-            fused = ops.tp_fused.get_context(group) if x.is_cuda and ops.tp_fused.ENABLED else None
-            if fused is not None:
-                logz, loss = fused.ce_combine(local_max, local_sumexp, local_tgt)  # tp reduction by peer loads inside the kernel
-            else:
-                gmax = local_max.clone()
-                dist.all_reduce(gmax, op=dist.ReduceOp.MAX, group=group)
-                packed = torch.stack([local_sumexp * torch.exp(local_max - gmax), local_tgt])
-                dist.all_reduce(packed, op=dist.ReduceOp.SUM, group=group)
-                logz = gmax + torch.log(packed[0])
-                loss = logz - packed[1]
-        if z is None and z_loss_coef > 0:
-            z = z_loss_coef * logz.square()
+        loss, z, x2, tgt, logz, vocab_start = _linear_cross_entropy_forward(x, weight, target, group, z_loss_coef)
         ctx.save_for_backward(x2, weight, tgt, logz)
         ctx.vocab_start, ctx.shape, ctx.z = vocab_start, x.shape, z_loss_coef
-        return loss.view(lead), (z.view(lead) if z is not None else None)
+        return loss, z
 
     @staticmethod
     @once_differentiable
@@ -350,9 +355,7 @@ def linear_cross_entropy(x, weight, target, group: Optional[dist.ProcessGroup] =
 
     A target outside the vocabulary counts as a class of score 0 without gradient, as in ``sharded_cross_entropy``: multiply such
     rows by a mask.  On CUDA: bf16, H a multiple of 64 (anything else raises ValueError); one level of differentiation."""
-    _check_linear_cross_entropy(x, weight, target, group)
-    loss, _ = _LinearCrossEntropy.apply(x, weight, target, group, 0.0)
-    return loss
+    return linear_cross_entropy_with_z_loss(x, weight, target, group, 0.0)[0]
 
 
 def linear_cross_entropy_with_z_loss(x, weight, target, group: Optional[dist.ProcessGroup] = None, z_loss_coef: float = 1e-4):
@@ -360,7 +363,9 @@ def linear_cross_entropy_with_z_loss(x, weight, target, group: Optional[dist.Pro
     _check_linear_cross_entropy(x, weight, target, group)
     if z_loss_coef < 0:
         raise ValueError(f"z_loss_coef must not be negative, got {z_loss_coef}")
-    return _LinearCrossEntropy.apply(x, weight, target, group, float(z_loss_coef))
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
+        return _LinearCrossEntropy.apply(x, weight, target, group, float(z_loss_coef))
+    return _linear_cross_entropy_forward(x, weight, target, group, float(z_loss_coef))[:2]
 
 
 __all__ = [
