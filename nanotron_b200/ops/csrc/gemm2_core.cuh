@@ -33,9 +33,8 @@ constexpr int P_B_BYTES = P_HALF_N * P_BLOCK_K * 2;   // 16 KiB
 constexpr int P_STAGE_BYTES = P_A_BYTES + P_B_BYTES;
 constexpr int P_EPI_WARPS = 4;
 constexpr int P_EPI_BUF = 32 * 128;
-constexpr int P_EPI_BYTES = P_EPI_WARPS * 2 * P_EPI_BUF;
 constexpr int P_THREADS = 32 * (2 + P_EPI_WARPS);
-constexpr int P_SMEM = P_MAX_STAGES * P_STAGE_BYTES + P_EPI_BYTES + 1024 + 512;
+constexpr int P_SMEM = P_MAX_STAGES * P_STAGE_BYTES + P_EPI_WARPS * 2 * P_EPI_BUF + 1024 + 512;
 
 enum POut { P_OUT_BF16 = 0, P_OUT_F32 = 1, P_OUT_F32_ACCUM = 2, P_OUT_PEER_BF16 = 3, P_OUT_CE_STATS = 4, P_OUT_CE_GRAD = 5 };
 
@@ -51,7 +50,7 @@ struct PCeArgs {
   const int64_t* target = nullptr;  // [M] class of every row, in the numbering in which column 0 of this product is `col0`
   int64_t col0 = 0;
   // P_OUT_CE_STATS: nothing but these leaves the kernel
-  float2* part = nullptr;           // [tiles_n][M] (largest score, sum exp(score - largest)) of every 256-column tile
+  float2* part = nullptr;           // [tiles_n * EW / 4][M] (largest score, sum exp(score - largest)) of every 1024 / EW columns
   float* tgt = nullptr;             // [M] the target's score, written where the target is one of this product's columns
   // P_OUT_CE_GRAD: D = coef * exp(score - logz) - g * [column is the target], zero in the padding columns of D
   const float* logz = nullptr;
@@ -223,16 +222,20 @@ __device__ __forceinline__ void p_ce_gradient(uint32_t (&r)[32], int valid, int 
   }
 }
 
-template <bool A_MN, bool B_MN, int OUT, int P_STAGES, class EXT = PPlain>
-__global__ void __launch_bounds__(P_THREADS, 1)
+// EW: epilogue warps per CTA, 4 (each takes 32 rows), or with P_OUT_CE_STATS, which stages nothing in shared memory, 8 (each takes 32
+// rows and half of the columns).
+template <bool A_MN, bool B_MN, int OUT, int P_STAGES, class EXT = PPlain, int EW = P_EPI_WARPS>
+__global__ void __launch_bounds__(32 * (2 + EW), 1)
 gemm2_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b, const __grid_constant__ CUtensorMap tmap_d,
                      int M, int N, int K, int band, int* __restrict__ status, const __grid_constant__ PFuse fuse, const __grid_constant__ PPeerMaps pmaps,
                      const __grid_constant__ PSched sched, const __grid_constant__ CUtensorMap tmap_ws, const __grid_constant__ CUtensorMap tmap_al,
                      const __grid_constant__ EXT ext) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* epi_smem = smem + P_MAX_STAGES * P_STAGE_BYTES;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(epi_smem + P_EPI_BYTES);
+  constexpr int EPI_BYTES = OUT == P_OUT_CE_STATS ? 0 : EW * 2 * P_EPI_BUF;
+  static_assert(P_STAGES * P_STAGE_BYTES + EPI_BYTES + 1024 + 512 <= P_SMEM && P_STAGES <= P_MAX_STAGES && (EW == 4 || (EW == 8 && OUT == P_OUT_CE_STATS)), "shared memory of a launch");
+  uint8_t* epi_smem = smem + P_STAGES * P_STAGE_BYTES;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(epi_smem + EPI_BYTES);
   uint64_t* full_bar = bars;                       // [STAGES]  (leader) both CTAs' loads of the stage have landed
   uint64_t* empty_bar = bars + 2 * P_MAX_STAGES;       // [STAGES]  the MMAs that read this stage are done
   uint64_t* tmem_full = bars + 3 * P_MAX_STAGES;       // [2]
@@ -256,7 +259,7 @@ gemm2_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
     }
     for (int b = 0; b < 2; b++) {
       ptx::mbar_init(&tmem_full[b], 1);  // leader: the MMA commit; peer: the remote arrive that forwards it
-      ptx::mbar_init(&tmem_empty[b], 2 * P_EPI_WARPS);
+      ptx::mbar_init(&tmem_empty[b], 2 * EW);
     }
     *abort_flag = 0;
     ptx::fence_barrier_init();
@@ -411,8 +414,10 @@ gemm2_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
           if (rel >= 0 && rel < cols) t = static_cast<int>(rel);
         }
         float m = -INFINITY, s = 0.f;
+        constexpr int PARTS = EW / 4, PART_CHUNKS = P_BLOCK_N / 32 / PARTS;
+        const int part = (warp - 2) >> 2;
 #pragma unroll 1
-        for (int c = 0; c < P_BLOCK_N / 32 && c * 32 < cols; c++) {
+        for (int c = part * PART_CHUNKS; c < (part + 1) * PART_CHUNKS && c * 32 < cols; c++) {
           uint32_t r0[32];
           ptx::tmem_ld_32x32(taddr + c * 32, r0);
           ptx::tmem_ld_wait();
@@ -424,7 +429,7 @@ gemm2_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
               if (j == tj) ext.tgt[row] = __uint_as_float(r0[j]);
           }
         }
-        if (row < M) ext.part[static_cast<int64_t>(tc.n_blk) * M + row] = make_float2(m, s);
+        if (row < M) ext.part[static_cast<int64_t>(tc.n_blk * PARTS + part) * M + row] = make_float2(m, s);
       } else {
       float ce_lz = 0.f, ce_coef = 0.f, ce_g = 0.f;
       int ce_t = -1, ce_cols = 0;

@@ -4,7 +4,7 @@
 //   d[t,v] = coef[t] exp(l[t,v] - logZ[t]) - g[t] [v == y_t]             dx = d w        dw = d^T x
 //
 // Forward: one GEMM over the whole vocabulary on CTA pairs (gemm2_core.cuh) whose epilogue keeps, per token and 256-column tile, only
-// (largest score, sum of exponentials); a small kernel joins the tiles of a token.  Scores never leave the tensor memory, and they
+// (largest score, sum of exponentials); a small kernel joins the half tiles of a token.  Scores never leave the tensor memory, and they
 // are used in fp32 (logits written in bf16 are off by up to 2^-9 of their value, several percent of a probability).
 // Backward: the vocabulary is cut into pieces; for each piece the scores are computed again, the epilogue turns them into d (bf16,
 // one rounding), and two plain products take d to dx (summed over the pieces in fp32) and to the piece's rows of dw.  Only one
@@ -93,12 +93,224 @@ __global__ void __launch_bounds__(256) ce_scale_cast_kernel(const float* __restr
   }
 }
 
+// ------------------------------------------------------------------------------------------------ a few tokens
+// Scores of up to 16 tokens: the work is reading the weight once.  A CTA takes 32 whole rows at a time, one contiguous piece of the weight,
+// and neighbouring CTAs neighbouring pieces; the 64-column blocks of the rows are dealt to eight warps, each with a ring of TMA loads of
+// its own, so no warp waits for another but at the end of the 32 rows.  1 x 2048 x 128256: 88 us, 6.0 TB/s (GEMM kernel 150 us); blocks of
+// 16 rows took 129 us, bound by the turn of a warp's loop (wait, read, four dependent products, next load) rather than by memory.
+//
+// With so few tokens the products are small: mma.sync m16n8k16, 16 weight rows x 8 tokens (bound by the
+// loads, not by this tensor path).  A lane reads 16 consecutive columns of a row
+// as two 16-byte words and feeds them to four products; the columns of a product are then a permutation of the block's, the same one
+// for weight and tokens, which a sum over columns does not see.  With the 128-byte swizzle of the loads these reads are free of bank
+// conflicts (lane t of a row takes words 2t, 2t + 1; eight lanes cover two rows and, after the swizzle, all eight word columns).
+constexpr int FEW_WARPS = 8;
+constexpr int FEW_ROWS = 32;
+constexpr int FEW_SLOT = FEW_ROWS * 128;  // bytes of one 32 x 64 block
+constexpr int FEW_MAX_TOKENS = 16;
+constexpr int FEW_MAX_STAGES = 8;
+constexpr int FEW_SMEM = 227 * 1024;
+
+struct FewLayout {  // of the dynamic shared memory, from a 1024-byte boundary on
+  int x_bytes, red_bytes, stages;
+};
+// NT: groups of 8 tokens.  Partial sums of the warps go through two buffers (one CTA barrier per 32 rows).
+__host__ __device__ inline FewLayout few_layout(int nt, int k_blocks) {
+  FewLayout l;
+  l.x_bytes = k_blocks * nt * 1024;
+  l.red_bytes = 2 * FEW_WARPS * FEW_ROWS * 8 * nt * 4;
+  const int left = FEW_SMEM - 2048 - l.x_bytes - l.red_bytes;
+  l.stages = left / (FEW_WARPS * FEW_SLOT);
+  if (l.stages > FEW_MAX_STAGES) l.stages = FEW_MAX_STAGES;
+  return l;
+}
+
+__device__ __forceinline__ void few_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// 16-byte word `word` of row `row` of a block whose rows are 128 bytes, swizzled by the load
+__device__ __forceinline__ uint4 few_word(const uint8_t* block, int row, int word) {
+  return *reinterpret_cast<const uint4*>(block + row * 128 + ((word ^ (row & 7)) << 4));
+}
+
+// GRAD false: part[blockIdx.x][T] = (largest, sum of exponentials) of the rows this CTA saw, and the targets' scores.  GRAD true:
+// d [T, V] at pitch ldd, columns up to `width` written.
+template <int NT, bool GRAD>
+__global__ void __launch_bounds__(FEW_WARPS * 32, 1)
+ce_few_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w, int T, int V, int k_blocks, PCeArgs args, __nv_bfloat16* __restrict__ d,
+              int64_t ldd, int width, int* __restrict__ status) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const FewLayout lay = few_layout(NT, k_blocks);
+  uint8_t* xs = smem;
+  uint8_t* ring = xs + lay.x_bytes;
+  float* red = reinterpret_cast<float*>(ring + lay.stages * FEW_WARPS * FEW_SLOT);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(red) + lay.red_bytes);  // [0]: tokens; then [warp][stage]
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + 1 + FEW_WARPS * FEW_MAX_STAGES);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = lane >> 2, t = lane & 3;
+  const int groups = ((GRAD ? width : V) + FEW_ROWS - 1) / FEW_ROWS;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 1 + FEW_WARPS * FEW_MAX_STAGES; i++) ptx::mbar_init(&bars[i], 1);
+    *abort_flag = 0;
+    ptx::fence_barrier_init();
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    ptx::mbar_expect_tx(&bars[0], lay.x_bytes);
+    for (int kb = 0; kb < k_blocks; kb++) ptx::tma_load_2d(xs + kb * NT * 1024, &tmap_x, &bars[0], kb * 64, 0);
+  }
+  // this warp's blocks, in order: for each of the CTA's groups, blocks warp, warp + 8, ...
+  const int per_group = k_blocks > warp ? (k_blocks - warp + FEW_WARPS - 1) / FEW_WARPS : 0;
+  const int my_groups = groups > static_cast<int>(blockIdx.x) ? (groups - static_cast<int>(blockIdx.x) + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x) : 0;
+  const int total = per_group * my_groups;
+  uint64_t* my_bars = bars + 1 + warp * FEW_MAX_STAGES;
+  uint8_t* my_ring = ring + warp * lay.stages * FEW_SLOT;
+  int next = 0, next_slot = 0, next_kb = warp, next_group = blockIdx.x;  // the next block to load (lane 0)
+  auto issue = [&]() {
+    ptx::mbar_expect_tx(&my_bars[next_slot], FEW_SLOT);
+    ptx::tma_load_2d(my_ring + next_slot * FEW_SLOT, &tmap_w, &my_bars[next_slot], next_kb * 64, next_group * FEW_ROWS);
+    next++;
+    if (++next_slot == lay.stages) next_slot = 0;
+    next_kb += FEW_WARPS;
+    if (next_kb >= k_blocks) next_kb = warp, next_group += gridDim.x;
+  };
+  if (lane == 0)
+    while (next < total && next < lay.stages) issue();
+  bool ok = __all_sync(0xffffffffu, ptx::mbar_wait(&bars[0], 0, abort_flag));
+
+  // thread -> (row, token) of the 32 x 8 NT scores, for the epilogue
+  constexpr int OWN = (FEW_ROWS * 8 * NT + FEW_WARPS * 32 - 1) / (FEW_WARPS * 32);
+  float run_m[OWN], run_s[OWN], e_lz[OWN], e_coef[OWN], e_g[OWN];
+  int e_t[OWN];
+#pragma unroll
+  for (int o = 0; o < OWN; o++) {
+    run_m[o] = -INFINITY;
+    run_s[o] = e_lz[o] = e_coef[o] = e_g[o] = 0.f;
+    e_t[o] = -1;
+    const int token = (threadIdx.x + o * FEW_WARPS * 32) / FEW_ROWS;
+    if (token < T) {
+      const int64_t rel = args.target[token] - args.col0;
+      if (rel >= 0 && rel < V) e_t[o] = static_cast<int>(rel);
+      if (GRAD) {
+        e_lz[o] = args.logz[token] * P_LOG2E;
+        e_coef[o] = args.coef[token];
+        e_g[o] = args.g[token];
+      }
+    }
+  }
+
+  int slot = 0, buf = 0;
+  uint32_t phase = 0;
+  for (int group = blockIdx.x; group < groups; group += gridDim.x) {
+    float acc[2][NT][4];
+#pragma unroll
+    for (int n = 0; n < NT; n++)
+#pragma unroll
+      for (int j = 0; j < 4; j++) acc[0][n][j] = acc[1][n][j] = 0.f;
+    for (int kb = warp; kb < k_blocks && ok; kb += FEW_WARPS) {
+      if (!__all_sync(0xffffffffu, ptx::mbar_wait(&my_bars[slot], phase, abort_flag))) { ok = false; break; }
+      const uint8_t* blk = my_ring + slot * FEW_SLOT;
+      uint4 w[2][4];  // [rows 0..15 | 16..31][row g: words 2t, 2t + 1; row g + 8: the same]
+#pragma unroll
+      for (int m = 0; m < 2; m++) {
+        w[m][0] = few_word(blk, m * 16 + g, 2 * t);
+        w[m][1] = few_word(blk, m * 16 + g, 2 * t + 1);
+        w[m][2] = few_word(blk, m * 16 + g + 8, 2 * t);
+        w[m][3] = few_word(blk, m * 16 + g + 8, 2 * t + 1);
+      }
+#pragma unroll
+      for (int n = 0; n < NT; n++) {
+        const uint8_t* xb = xs + (kb * NT + n) * 1024;
+        const uint4 b0 = few_word(xb, g, 2 * t), b1 = few_word(xb, g, 2 * t + 1);
+#pragma unroll
+        for (int m = 0; m < 2; m++) few_mma(acc[m][n], w[m][0].x, w[m][2].x, w[m][0].y, w[m][2].y, b0.x, b0.y);
+#pragma unroll
+        for (int m = 0; m < 2; m++) few_mma(acc[m][n], w[m][0].z, w[m][2].z, w[m][0].w, w[m][2].w, b0.z, b0.w);
+#pragma unroll
+        for (int m = 0; m < 2; m++) few_mma(acc[m][n], w[m][1].x, w[m][3].x, w[m][1].y, w[m][3].y, b1.x, b1.y);
+#pragma unroll
+        for (int m = 0; m < 2; m++) few_mma(acc[m][n], w[m][1].z, w[m][3].z, w[m][1].w, w[m][3].w, b1.z, b1.w);
+      }
+      __syncwarp();  // every lane's reads of the block have been consumed by the products above
+      if (lane == 0 && next < total) issue();
+      if (++slot == lay.stages) slot = 0, phase ^= 1;
+    }
+    // the warps' shares of the 32 x 8 NT scores, [token][row]
+    float* out = red + (buf * FEW_WARPS + warp) * FEW_ROWS * 8 * NT;
+#pragma unroll
+    for (int n = 0; n < NT; n++)
+#pragma unroll
+      for (int m = 0; m < 2; m++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) out[(n * 8 + 2 * t + (j & 1)) * FEW_ROWS + m * 16 + g + (j & 2) * 4] = acc[m][n][j];
+    if (__syncthreads_or(!ok)) {  // the same answer in every thread
+      ok = false;
+      break;
+    }
+#pragma unroll
+    for (int o = 0; o < OWN; o++) {
+      const int i = threadIdx.x + o * FEW_WARPS * 32;
+      const int token = i / FEW_ROWS, v = group * FEW_ROWS + i % FEW_ROWS;
+      if (token >= T) continue;
+      float sc = 0.f;
+#pragma unroll
+      for (int w = 0; w < FEW_WARPS; w++) sc += red[(buf * FEW_WARPS + w) * FEW_ROWS * 8 * NT + i];
+      if (GRAD) {
+        if (v < width) {
+          float p = v < V ? e_coef[o] * p_ex2(fmaf(sc, P_LOG2E, -e_lz[o])) : 0.f;
+          if (v == e_t[o]) p -= e_g[o];
+          d[token * ldd + v] = __float2bfloat16_rn(p);
+        }
+      } else if (v < V) {
+        if (v == e_t[o]) args.tgt[token] = sc;
+        const float nm = fmaxf(run_m[o], sc);
+        const float base = nm == -INFINITY ? 0.f : nm * P_LOG2E;
+        run_s[o] = run_s[o] * p_ex2(fmaf(run_m[o], P_LOG2E, -base)) + p_ex2(fmaf(sc, P_LOG2E, -base));
+        run_m[o] = nm;
+      }
+    }
+    buf ^= 1;
+  }
+  if (!ok) {  // leave no load in flight behind (bounded)
+    if (lane == 0) {
+      const uint64_t t0 = ptx::globaltimer();
+      for (int j = next > lay.stages ? next - lay.stages : 0; j < next; j++)
+        while (!ptx::mbar_try_wait(&my_bars[j % lay.stages], (j / lay.stages) & 1) && ptx::globaltimer() - t0 < NTB_WAIT_LIMIT_NS) {}
+      if (warp == 0)
+        while (!ptx::mbar_try_wait(&bars[0], 0) && ptx::globaltimer() - t0 < NTB_WAIT_LIMIT_NS) {}
+    }
+    if (threadIdx.x == 0 && status) atomicExch(status, NTB_ERR_TIMEOUT);
+    return;
+  }
+  if (!GRAD) {
+#pragma unroll
+    for (int o = 0; o < OWN; o++) {
+      // the 32 rows of a token sit in the 32 lanes of a warp
+      float m = run_m[o], s = run_s[o];
+#pragma unroll
+      for (int k = 16; k > 0; k >>= 1) {
+        const float om = __shfl_xor_sync(0xffffffffu, m, k), os = __shfl_xor_sync(0xffffffffu, s, k);
+        const float nm = fmaxf(m, om);
+        const float base = nm == -INFINITY ? 0.f : nm * P_LOG2E;
+        s = s * p_ex2(fmaf(m, P_LOG2E, -base)) + os * p_ex2(fmaf(om, P_LOG2E, -base));
+        m = nm;
+      }
+      const int i = threadIdx.x + o * FEW_WARPS * 32;
+      if (i % FEW_ROWS == 0 && i / FEW_ROWS < T) args.part[static_cast<int64_t>(blockIdx.x) * T + i / FEW_ROWS] = make_float2(m, s);
+    }
+  }
+}
+
 template <class K>
-int ce_configure(K kern, bool (&done)[64]) {
+int ce_configure(K kern, bool (&done)[64], int smem) {
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return NTB_ERR_LAUNCH;
   if (!done[dev]) {
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, P_SMEM) != cudaSuccess) {
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) {
       cudaGetLastError();
       return NTB_ERR_LAUNCH;
     }
@@ -114,18 +326,24 @@ int ce_band(int M, int K) {
   return band > tiles_m ? tiles_m : band;
 }
 
+// The statistics' epilogue is the longest (an exponential per score and nothing to store) and the only one that needs no shared memory:
+// eight warps share it (2048 x 256 x 32000: 60 -> 51 us, 2047 x 768 x 50257: 115 -> 109 us; level at H = 4096).  The gradient's with
+// eight warps and one operand stage less measured level (2047 x 768 x 50257: 337 us for the three products against 334) and keeps four.
+constexpr int CE_STATS_WARPS = 8;
+
 template <bool A_MN, bool B_MN, int OUT, class EXT>
 int ce_launch(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& td, int M, int N, int K, const PSched& sched, const CUtensorMap& tws, const EXT& ext,
               int* status, int num_sms, cudaStream_t stream) {
-  auto kern = gemm2_tcgen05_kernel<A_MN, B_MN, OUT, P_MAX_STAGES, EXT>;
+  constexpr int EW = OUT == P_OUT_CE_STATS ? CE_STATS_WARPS : P_EPI_WARPS;
+  auto kern = gemm2_tcgen05_kernel<A_MN, B_MN, OUT, P_MAX_STAGES, EXT, EW>;
   static bool done[64] = {};
-  if (int rc = ce_configure(kern, done)) return rc;
+  if (int rc = ce_configure(kern, done, P_SMEM)) return rc;
   static const PPeerMaps no_maps = {};
   int pairs = num_sms / 2;
   if (sched.total_units < pairs) pairs = sched.total_units;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(2 * pairs), 1, 1);
-  cfg.blockDim = dim3(P_THREADS, 1, 1);
+  cfg.blockDim = dim3(32 * (2 + EW), 1, 1);
   cfg.dynamicSmemBytes = P_SMEM;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
@@ -152,35 +370,79 @@ PSched ce_whole_tiles(int M, int N, int K, bool& fits) {
   return sc;
 }
 
+// Groups of 8 tokens of the few-token kernel, 0: the GEMM kernel.  The tokens' padded copy may take up to 128 KB, the rings the rest.
+// Forward pass, us, this kernel | GEMM kernel: 1 x 2048 x 128256 88 | 150, 16 x 4096 x 128256 177 | 199, 1 x 8192 x 128256 330 | 372; with four
+// groups 32 x 1024 x 128256 took 82 against 80, so more than 16 tokens go to the GEMM kernel.
+int ce_few_groups(int T, int H) {
+  if (T > FEW_MAX_TOKENS) return 0;
+  const int nt = (T + 7) / 8;
+  return static_cast<int64_t>(nt) * 8 * H <= 65536 ? nt : 0;
+}
+
+bool few_map(CUtensorMap* m, const void* ptr, int64_t rows, int64_t k, int64_t ld, int box_rows) {
+  cuuint64_t dims[2] = {(cuuint64_t)k, (cuuint64_t)rows};
+  cuuint64_t strides[1] = {(cuuint64_t)ld * 2};
+  cuuint32_t box[2] = {64, (cuuint32_t)box_rows};
+  cuuint32_t es[2] = {1, 1};
+  return p_get_encode()(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(ptr), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+int few_grid(int rows, int num_sms) {
+  const int groups = (rows + FEW_ROWS - 1) / FEW_ROWS;
+  return groups < num_sms ? groups : num_sms;
+}
+
+template <int NT, bool GRAD>
+int few_launch(const void* x, int64_t ldx, const void* w, int64_t ldw, int T, int V, int H, const PCeArgs& a, void* d, int64_t ldd, int width, int* status, int num_sms,
+               cudaStream_t stream) {
+  auto kern = ce_few_kernel<NT, GRAD>;
+  static bool done[64] = {};
+  if (int rc = ce_configure(kern, done, FEW_SMEM)) return rc;
+  CUtensorMap tx, tw;
+  if (!few_map(&tx, x, T, H, ldx, NT * 8) || !few_map(&tw, w, V, H, ldw, FEW_ROWS)) return NTB_ERR_ARG;
+  kern<<<few_grid(GRAD ? width : V, num_sms), FEW_WARPS * 32, FEW_SMEM, stream>>>(tx, tw, T, V, H / 64, a, static_cast<__nv_bfloat16*>(d), ldd, width, status);
+  return ntb_check_launch();
+}
+template <bool GRAD>
+int few_dispatch(int nt, const void* x, int64_t ldx, const void* w, int64_t ldw, int T, int V, int H, const PCeArgs& a, void* d, int64_t ldd, int width, int* status, int num_sms,
+                 cudaStream_t stream) {
+  if (nt == 1) return few_launch<1, GRAD>(x, ldx, w, ldw, T, V, H, a, d, ldd, width, status, num_sms, stream);
+  return few_launch<2, GRAD>(x, ldx, w, ldw, T, V, H, a, d, ldd, width, status, num_sms, stream);
+}
+
 bool ce_operand_ok(const void* p, int64_t ld) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld % 64 == 0; }
 
 int ce_stats(const void* x, int64_t ldx, const void* w, int64_t ldw, const int64_t* target, int64_t vocab_start, int T, int V, int H, void* part, float* tgt, int* status,
              int num_sms, cudaStream_t stream) {
-  bool fits;
-  const PSched sched = ce_whole_tiles(T, V, H, fits);
-  CUtensorMap ta, tb;
-  if (!fits || !p_map_kmajor(&ta, x, T, H, ldx) || !p_map_kmajor(&tb, w, V, H, ldw)) return NTB_ERR_ARG;
   PCeArgs a;
   a.target = target;
   a.col0 = vocab_start;
   a.part = static_cast<float2*>(part);
   a.tgt = tgt;
+  if (const int nt = ce_few_groups(T, H)) return few_dispatch<false>(nt, x, ldx, w, ldw, T, V, H, a, nullptr, 0, 0, status, num_sms, stream);
+  bool fits;
+  const PSched sched = ce_whole_tiles(T, V, H, fits);
+  CUtensorMap ta, tb;
+  if (!fits || !p_map_kmajor(&ta, x, T, H, ldx) || !p_map_kmajor(&tb, w, V, H, ldw)) return NTB_ERR_ARG;
   return ce_launch<false, false, P_OUT_CE_STATS>(ta, tb, ta, T, V, H, sched, ta, a, status, num_sms, stream);
 }
 
 // d [T, V] at pitch ldd; the columns up to V rounded up to 64 are written (zeros behind V).
 int ce_dlogits(const void* x, int64_t ldx, const void* w, int64_t ldw, const int64_t* target, int64_t vocab_start, const float* logz, const float* coef, const float* gn,
                int T, int V, int H, void* d, int64_t ldd, int* status, int num_sms, cudaStream_t stream) {
-  bool fits;
-  const PSched sched = ce_whole_tiles(T, V, H, fits);
-  CUtensorMap ta, tb, td;
-  if (!fits || !p_map_kmajor(&ta, x, T, H, ldx) || !p_map_kmajor(&tb, w, V, H, ldw) || !p_map_out(&td, d, T, (static_cast<int64_t>(V) + 63) / 64 * 64, ldd, false)) return NTB_ERR_ARG;
+  const int64_t width = (static_cast<int64_t>(V) + 63) / 64 * 64;
   PCeArgs a;
   a.target = target;
   a.col0 = vocab_start;
   a.logz = logz;
   a.coef = coef;
   a.g = gn;
+  if (const int nt = ce_few_groups(T, H)) return few_dispatch<true>(nt, x, ldx, w, ldw, T, V, H, a, d, ldd, static_cast<int>(width), status, num_sms, stream);
+  bool fits;
+  const PSched sched = ce_whole_tiles(T, V, H, fits);
+  CUtensorMap ta, tb, td;
+  if (!fits || !p_map_kmajor(&ta, x, T, H, ldx) || !p_map_kmajor(&tb, w, V, H, ldw) || !p_map_out(&td, d, T, width, ldd, false)) return NTB_ERR_ARG;
   return ce_launch<false, false, P_OUT_CE_GRAD>(ta, tb, td, T, V, H, sched, ta, a, status, num_sms, stream);
 }
 
@@ -273,13 +535,14 @@ int ce_dw(const void* d, int64_t ldd, const void* x, int64_t ldx, void* dw, int6
 }  // namespace
 
 // x [T, H] and w [V, H] bf16, rows 16-byte aligned at pitches ldx, ldw (multiples of 64), H a multiple of 64; target int64 [T]; this
-// rank's rows of the vocabulary start at vocab_start.  part: fp32 scratch, (ceil(V / 256) * 2 + 1) * T elements, 8-byte aligned.
+// rank's rows of the vocabulary start at vocab_start.  part: fp32 scratch, (max(ceil(V / 256) * 4, 2 * min(ceil(V / 32), num_sms)) + 1) * T elements, 8-byte aligned.
 // out: fp32 planes of T: with finish, logZ, loss and (z_coef > 0) z_coef logZ^2; without, the three numbers that vocabulary shards
 // exchange: largest score, sum of exp(score - largest), the target's score or 0.
 NTB_EXPORT int ntb_linear_ce_forward(const void* x, int64_t ldx, const void* w, int64_t ldw, const int64_t* target, int64_t vocab_start, int T, int V, int H, float* part,
                                      float* out, int finish, float z_coef, int* status, int num_sms, cudaStream_t stream) {
   if (T <= 0 || V <= 0 || H <= 0 || H % 64 || !ce_operand_ok(x, ldx) || !ce_operand_ok(w, ldw) || (reinterpret_cast<uintptr_t>(part) & 7) || num_sms < 2 || !p_get_encode()) return NTB_ERR_ARG;
-  const int tiles = (V + P_BLOCK_N - 1) / P_BLOCK_N;
+  // partial statistics per token: one of every half tile (the last may have no columns: (-inf, 0)), or one of every CTA
+  const int tiles = ce_few_groups(T, H) ? few_grid(V, num_sms) : (V + P_BLOCK_N - 1) / P_BLOCK_N * (CE_STATS_WARPS / 4);
   float* tgt = part + static_cast<int64_t>(tiles) * 2 * T;
   const int rc = ce_stats(x, ldx, w, ldw, target, vocab_start, T, V, H, part, tgt, status, num_sms, stream);
   if (rc != NTB_OK) return rc;

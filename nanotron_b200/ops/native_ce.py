@@ -6,6 +6,7 @@ current stream of the tensors' device; scratch comes from torch's allocator per 
 from __future__ import annotations
 
 from ctypes import c_float, c_int, c_int64, c_void_p
+from itertools import accumulate
 from typing import Optional
 
 import torch
@@ -59,10 +60,11 @@ def forward(x2: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, vocab_
     (T, H), V, dev = x2.shape, weight.shape[0], x2.device
     with native.on_device(dev):
         status = _status(dev)
-        part = torch.empty(((V + 255) // 256 * 2 + 1) * T, dtype=torch.float32, device=dev)  # per tile two numbers, and the target's score
+        sms = native_gemm._sms(dev)
+        part = torch.empty((max((V + 255) // 256 * 4, 2 * sms) + 1) * T, dtype=torch.float32, device=dev)  # per part two numbers, and the target's score
         out = torch.empty((3 if z_coef > 0 or not finish else 2, T), dtype=torch.float32, device=dev)
         native._check(native.lib().ntb_linear_ce_forward(x2.data_ptr(), x2.stride(0), weight.data_ptr(), weight.stride(0), target.data_ptr(), vocab_start, T, V, H, part.data_ptr(),
-                                                         out.data_ptr(), int(finish), z_coef, status.data_ptr(), native_gemm._sms(dev), native.raw_stream(x2)), "linear_ce_forward", launches=2)
+                                                         out.data_ptr(), int(finish), z_coef, status.data_ptr(), sms, native.raw_stream(x2)), "linear_ce_forward", launches=2)
     return out
 
 
@@ -82,17 +84,19 @@ def backward(x2, weight, target, logz, g, gz: Optional[torch.Tensor], z_coef: fl
     with native.on_device(dev):
         width = piece_width(T, V)
         pitch = (min(width, V) + 63) // 64 * 64
-        d = torch.empty((T, pitch), dtype=torch.bfloat16, device=dev)
-        rows = torch.empty(2 * T + 1, dtype=torch.float32, device=dev)
         dx = torch.empty((T, H), dtype=torch.bfloat16, device=dev) if need_dx else None
-        acc = torch.empty((T, H), dtype=torch.float32, device=dev) if need_dx and width < V else None
         split = L.ntb_linear_ce_dx_split(T, min(width, V), H, sms) if need_dx else 1
-        ws = torch.empty(split * ((T + 255) // 256) * ((H + 255) // 256) * 65536, dtype=torch.float32, device=dev) if split > 1 else None
+        # scratch, in fp32 words with every part on a 1024-byte boundary: d (bf16 [T, pitch]), coefficients (2 T + 1), dx over several
+        # pieces (fp32 [T, H]), partial sums of a dx that is cut along the vocabulary
+        parts = [T * pitch // 2, 2 * T + 1, T * H if need_dx and width < V else 0, split * ((T + 255) // 256) * ((H + 255) // 256) * 65536 if split > 1 else 0]
+        ends = list(accumulate((n + 255) // 256 * 256 for n in parts))
+        scratch = torch.empty(ends[-1], dtype=torch.float32, device=dev)
+        d, rows, acc, ws = (scratch.data_ptr() + 4 * (e - (n + 255) // 256 * 256) if n else None for n, e in zip(parts, ends))
         dw = torch.empty((V, H), dtype=torch.bfloat16, device=dev) if need_dw and main_grad is None else None
         into = (main_grad if main_grad is not None else dw) if need_dw else None
         pieces = (V + width - 1) // width
         rc = L.ntb_linear_ce_backward(x2.data_ptr(), x2.stride(0), weight.data_ptr(), weight.stride(0), target.data_ptr(), vocab_start, logz.data_ptr(), g.data_ptr(), ptr(gz), z_coef,
-                                      T, V, H, width, d.data_ptr(), pitch, rows.data_ptr(), ptr(dx), ptr(acc), split, ptr(ws), ptr(into), into.stride(0) if need_dw else H,
+                                      T, V, H, width, d, pitch, rows, ptr(dx), acc, split, ws, ptr(into), into.stride(0) if need_dw else H,
                                       int(main_grad is not None), _status(dev).data_ptr(), sms, native.raw_stream(x2))
         native._check(rc, "linear_ce_backward", launches=1 + pieces * (1 + (1 + (split > 1)) * need_dx + need_dw) + (acc is not None))
     return dx, dw
