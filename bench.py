@@ -166,7 +166,7 @@ def build_config(args, world: int):
         logging=c.LoggingArgs(log_level="warning", log_level_replica="error", iteration_step_info_interval=10**9),
         tokens=c.TokensArgs(sequence_length=args.seq, train_steps=10**6, micro_batch_size=args.mbs, batch_accumulation_per_replica=args.accum),
         optimizer=c.OptimizerArgs(
-            optimizer_factory=c.AdamWOptimizerArgs(adam_eps=1e-8, adam_beta1=0.9, adam_beta2=0.95, torch_adam_is_fused=True),
+            optimizer_factory=c.AdamWOptimizerArgs(adam_eps=1e-8, adam_beta1=0.9, adam_beta2=0.95, torch_adam_is_fused=True, state_bits=getattr(args, "state_bits", 32)),
             zero_stage=zero, weight_decay=0.01, clip_grad=1.0, accumulate_grad_in_fp32=True, overlap_grad_reduce=not args.no_grad_overlap,
             learning_rate_scheduler=c.LRSchedulerArgs(learning_rate=3e-4, lr_warmup_steps=2, lr_decay_style="cosine", min_decay_lr=3e-5),
         ),
@@ -196,6 +196,7 @@ def run_native(args):
     ops.set_gemm(args.gemm)
     ops.set_attention(args.attention)
     ops.set_linear(args.linear)
+    ops.set_loss(args.loss)
     from nanotron_b200.ops import native_gemm
 
     native_gemm.set_variant(args.gemm_variant)
@@ -280,7 +281,7 @@ def run_native(args):
                 "pp_p2p": "NCCL send/recv on one lane per direction, asynchronous" if pp > 1 else "n/a",
                 "dp_step": ("in-tree NVLink kernels (reduce-scatter" + (" per layer during the last backward" if (trainer.fused_dp.buckets and not args.no_grad_overlap) else "") + " + AdamW + all-gather)") if getattr(trainer, "fused_dp", None) is not None else "NCCL", "fp32_grad_accum": True, "fp32_master_weights": True, "optimizer": "AdamW", "clip_grad": 1.0,
                 "recompute_layer": bool(args.recompute), "l2": "inputs larger than L2 (per-step working set is tens of GB); no explicit flush",
-                "gemm": ops._GEMM, "gemm_kernel": args.gemm_variant, "attention": ops._ATTN, "linear": ops.get_linear(),
+                "gemm": ops._GEMM, "gemm_kernel": args.gemm_variant, "attention": ops._ATTN, "linear": ops.get_linear(), "loss": ops.get_loss(), "optimizer_state_bits": args.state_bits,
             },
             "clocks": clocks,
             "e2e": {"value": e2e_value, "unit": "tokens/s", "ms_per_step": e2e_ms / args.steps, "h2d_bytes_per_step": 2 * args.mbs * args.seq * 8 * args.accum, "d2h_bytes_per_step": 4},
@@ -312,6 +313,8 @@ def main():
     ap.add_argument("--gemm", default="auto", choices=["auto", "tcgen05", "cublas"], help="auto / tcgen05: every linear-layer product on the in-tree tcgen05 kernels; cublas: library GEMMs (wgrad then needs a separate fp32 add)")
     ap.add_argument("--attention", default="auto", choices=["auto", "native", "sdpa"], help="auto / native: the in-tree tcgen05 flash-attention kernels; sdpa: library attention (comparison runs)")
     ap.add_argument("--linear", default="bf16", choices=["bf16", "fp8"], help="fp8: block-scaled fp8 operands (e4m3 forward, e5m2 gradients) for the linear-layer products")
+    ap.add_argument("--loss", default="logits", choices=["logits", "fused"], help="fused: cross entropy from the head's operands, no logits kept between forward and backward")
+    ap.add_argument("--state-bits", type=int, default=32, choices=[32, 8], help="bits of AdamW's running averages")
     ap.add_argument("--gemm-variant", default="pair", choices=["single", "pair"], help="in-tree GEMM kernel: one CTA per 128x256 tile, or CTA pairs (cta_group::2) per 256x256 tile")
     ap.add_argument("--layout", default=None, choices=["model", "dp"], help="model: tp / pp by GPU count (1: none, 2: tp2, 4: tp4, 8: tp4 x pp2), same global batch at every N; dp: data parallel over all GPUs with ZeRO-1")
     ap.add_argument("--tp", type=int, default=None, help="tensor-parallel size (sequence-parallel mode), overrides --layout; dp = gpus / (tp * pp)")
