@@ -60,9 +60,12 @@ struct AmHyper {
   float b1, omb1, b2, omb2, eps, inv_bc1, inv_sqrt_bc2;  // omb: 1 - b, rounded once from 64 bits (1.f - 0.999f is off by 2^-16); bc: 1 - b^t
   const float* grad_scale;
   uint32_t by4, by8;  // AmShift
+  float one;
 };
 
-// Two fp32 operations at a time, each rounded by itself (never contracted into a fused multiply-add).
+// Two fp32 operations at a time, each rounded by itself.  The sum is written as a fused multiply-add with a factor of 1 that the
+// compiler does not know: ptxas contracts mul.rn.f32x2 + add.rn.f32x2 into one fused operation (a quarter of the sums then differ in
+// their last bit from separately rounded ones, and some 3e-7 of the codes with them); a product by 1 leaves it nothing to contract.
 struct F2 {
   float x, y;
 };
@@ -71,9 +74,11 @@ __device__ __forceinline__ F2 mul_rn(F2 a, F2 b) {
   asm("{ .reg .b64 a, b, c; mov.b64 a, {%2, %3}; mov.b64 b, {%4, %5}; mul.rn.f32x2 c, a, b; mov.b64 {%0, %1}, c; }" : "=f"(c.x), "=f"(c.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   return c;
 }
-__device__ __forceinline__ F2 add_rn(F2 a, F2 b) {
+__device__ __forceinline__ F2 add_rn(F2 a, F2 b, float one) {
   F2 c;
-  asm("{ .reg .b64 a, b, c; mov.b64 a, {%2, %3}; mov.b64 b, {%4, %5}; add.rn.f32x2 c, a, b; mov.b64 {%0, %1}, c; }" : "=f"(c.x), "=f"(c.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  asm("{ .reg .b64 a, b, c, o; mov.b64 a, {%2, %3}; mov.b64 b, {%4, %5}; mov.b64 o, {%6, %6}; fma.rn.f32x2 c, a, o, b; mov.b64 {%0, %1}, c; }"
+      : "=f"(c.x), "=f"(c.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(one));
   return c;
 }
 
@@ -252,8 +257,8 @@ template <typename P, typename G, int BITS> struct AmBlock {
 #pragma unroll
       for (int j = 0; j < 4; j += 2) {
         const F2 gj = mul_rn(F2{g[j], g[j + 1]}, F2{gs, gs});
-        const F2 mj = add_rn(mul_rn(F2{m[j], m[j + 1]}, F2{b1, b1}), mul_rn(gj, F2{hy.omb1, hy.omb1}));
-        const F2 vj = add_rn(mul_rn(F2{v[j], v[j + 1]}, F2{b2, b2}), mul_rn(mul_rn(gj, gj), F2{hy.omb2, hy.omb2}));
+        const F2 mj = add_rn(mul_rn(F2{m[j], m[j + 1]}, F2{b1, b1}), mul_rn(gj, F2{hy.omb1, hy.omb1}), hy.one);
+        const F2 vj = add_rn(mul_rn(F2{v[j], v[j + 1]}, F2{b2, b2}), mul_rn(mul_rn(gj, gj), F2{hy.omb2, hy.omb2}), hy.one);
         m[j] = mj.x; m[j + 1] = mj.y;
         v[j] = vj.x; v[j + 1] = vj.y;
       }
@@ -444,7 +449,7 @@ NTB_EXPORT int ntb_adamw_multi(void* table, int count, int p_dtype, int g_dtype,
     const uintptr_t p = reinterpret_cast<uintptr_t>(t[i].p), g = reinterpret_cast<uintptr_t>(t[i].g), s = reinterpret_cast<uintptr_t>(t[i].m) | reinterpret_cast<uintptr_t>(t[i].v);
     t[i].vec = p % (p_dtype == NTB_F32 ? 16 : 8) == 0 && g % (g_dtype == NTB_F32 ? 16 : 8) == 0 && s % (bits == 32 ? 16 : 4) == 0 && reinterpret_cast<uintptr_t>(t[i].half) % 8 == 0;
   }
-  AmHyper hy = {b1, omb1, b2, omb2, eps, 1.f / bias_correction1, rsqrtf(bias_correction2), grad_scale, 16u, 256u};
+  AmHyper hy = {b1, omb1, b2, omb2, eps, 1.f / bias_correction1, rsqrtf(bias_correction2), grad_scale, 16u, 256u, 1.f};
   if (p_dtype == NTB_F32 && g_dtype == NTB_F32) return am_dispatch<float, float>(t, count, bits, hy, num_sms, stream);
   if (p_dtype == NTB_F32 && g_dtype == NTB_BF16) return am_dispatch<float, __nv_bfloat16>(t, count, bits, hy, num_sms, stream);
   if (p_dtype == NTB_BF16 && g_dtype == NTB_F32) return am_dispatch<__nv_bfloat16, float>(t, count, bits, hy, num_sms, stream);

@@ -333,6 +333,26 @@ def test_8_bit_states_equal_the_pytorch_form_over_steps(g_dtype):
 
 
 @gpu
+def test_8_bit_states_equal_the_pytorch_form_on_many_elements():
+    """A last bit of m or v changes a code with a chance of about 2^-20: 2^26 elements would show it if a share of the sums were rounded
+    otherwise (by a fused multiply-add, say)."""
+    n = 1 << 26
+    gen = torch.Generator(device=DEV).manual_seed(5)
+    g = torch.randn(n, generator=gen, device=DEV) * 1e-2
+    m, v = g * 0.3 + 1e-3 * torch.randn(n, generator=gen, device=DEV), (1e-2 * torch.randn(n, generator=gen, device=DEV)).square()
+    a = {"p": [torch.zeros(n, device=DEV)], "g": [g], "h": None}
+    (c, e), (k, f) = ops.q8_encode(m, True), ops.q8_encode(v, False)
+    a["m"], a["me"], a["v"], a["ve"] = [c], [e], [k], [f]
+    b = {key: [t.clone() for t in value] if value else None for key, value in a.items()}
+    scale = torch.tensor(0.83, device=DEV)
+    apply(a, 8, scale)
+    with ops.mode("torch"):
+        apply(b, 8, scale)
+    for key in ("m", "v", "me", "ve"):
+        assert torch.equal(a[key][0], b[key][0]), key
+
+
+@gpu
 @pytest.mark.parametrize("bits", [32, 8])
 @pytest.mark.parametrize("count", [24, 25, 384, 385, 800])
 def test_many_tensors(bits, count):
