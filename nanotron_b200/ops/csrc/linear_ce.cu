@@ -539,20 +539,21 @@ int ce_dw(const void* d, int64_t ldd, const void* x, int64_t ldx, void* dw, int6
 
 // x [T, H] and w [V, H] bf16, rows 16-byte aligned at pitches ldx, ldw (multiples of 64), H a multiple of 64; target int64 [T]; this
 // rank's rows of the vocabulary start at vocab_start.  part: fp32 scratch, (max(ceil(V / 256) * 4, 2 * min(ceil(V / 32), num_sms)) + 1) * T elements, 8-byte aligned.
-// out: fp32 planes of T: with finish, logZ, loss and (z_coef > 0) z_coef logZ^2; without, the three numbers that vocabulary shards
-// exchange: largest score, sum of exp(score - largest), the target's score or 0.
+// out0..2: fp32 [T]: with finish, logZ, loss and (z_coef > 0) z_coef logZ^2; without, the three numbers that vocabulary shards exchange:
+// largest score, sum of exp(score - largest), the target's score or 0.
 NTB_EXPORT int ntb_linear_ce_forward(const void* x, int64_t ldx, const void* w, int64_t ldw, const int64_t* target, int64_t vocab_start, int T, int V, int H, float* part,
-                                     float* out, int finish, float z_coef, int* status, int num_sms, cudaStream_t stream) {
-  if (T <= 0 || V <= 0 || H <= 0 || H % 64 || !ce_operand_ok(x, ldx) || !ce_operand_ok(w, ldw) || (reinterpret_cast<uintptr_t>(part) & 7) || num_sms < 2 || !p_get_encode()) return NTB_ERR_ARG;
+                                     float* out0, float* out1, float* out2, int finish, float z_coef, int* status, int num_sms, cudaStream_t stream) {
+  if (T <= 0 || V <= 0 || H <= 0 || H % 64 || !ce_operand_ok(x, ldx) || !ce_operand_ok(w, ldw) || (reinterpret_cast<uintptr_t>(part) & 7) || num_sms < 2 || !out0 || !out1 || (!out2 && (!finish || z_coef > 0.f)) ||
+      !p_get_encode())
+    return NTB_ERR_ARG;
   // partial statistics per token: one of every half tile (the last may have no columns: (-inf, 0)), or one of every CTA
   const int tiles = ce_few_groups(T, H) ? few_grid(V, num_sms) : (V + P_BLOCK_N - 1) / P_BLOCK_N * (CE_STATS_WARPS / 4);
   float* tgt = part + static_cast<int64_t>(tiles) * 2 * T;
   const int rc = ce_stats(x, ldx, w, ldw, target, vocab_start, T, V, H, part, tgt, status, num_sms, stream);
   if (rc != NTB_OK) return rc;
-  float *a = out, *b = out + T, *c = out + 2 * static_cast<int64_t>(T);
   ce_join_kernel<<<(T + CE_JOIN_ROWS - 1) / CE_JOIN_ROWS, CE_JOIN_ROWS * CE_JOIN_PARTS, 0, stream>>>(
-      reinterpret_cast<const float2*>(part), tgt, target, vocab_start, V, tiles, T, finish ? nullptr : a, finish ? nullptr : b, finish ? nullptr : c, finish ? a : nullptr,
-      finish ? b : nullptr, finish && z_coef > 0.f ? c : nullptr, z_coef);
+      reinterpret_cast<const float2*>(part), tgt, target, vocab_start, V, tiles, T, finish ? nullptr : out0, finish ? nullptr : out1, finish ? nullptr : out2,
+      finish ? out0 : nullptr, finish ? out1 : nullptr, finish && z_coef > 0.f ? out2 : nullptr, z_coef);
   return ntb_check_launch();
 }
 

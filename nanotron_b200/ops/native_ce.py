@@ -6,6 +6,7 @@ current stream of the tensors' device; scratch comes from torch's allocator per 
 from __future__ import annotations
 
 from ctypes import c_float, c_int, c_int64, c_void_p
+from functools import lru_cache
 from itertools import accumulate
 from typing import Optional
 
@@ -19,7 +20,7 @@ PIECE_MIN = 4096          # narrowest piece: below it the sums of dx over the pi
 
 def declare(L):
     L.ntb_linear_ce_forward.restype = c_int
-    L.ntb_linear_ce_forward.argtypes = [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int, c_int, c_int, c_void_p, c_void_p, c_int, c_float, c_void_p, c_int, c_void_p]
+    L.ntb_linear_ce_forward.argtypes = [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int, c_int, c_int] + [c_void_p] * 4 + [c_int, c_float, c_void_p, c_int, c_void_p]
     L.ntb_linear_ce_dx_split.restype = c_int
     L.ntb_linear_ce_dx_split.argtypes = [c_int] * 4
     L.ntb_linear_ce_backward.restype = c_int
@@ -53,19 +54,20 @@ def _status(device) -> torch.Tensor:
     return native_gemm.status_word(device)
 
 
-def forward(x2: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, vocab_start: int, finish: bool, z_coef: float = 0.0) -> torch.Tensor:
-    """fp32 planes [.., T]; ``finish``: logZ and loss of a whole vocabulary, and z_coef logZ^2 when that is positive; otherwise this
-    shard's largest score, sum of exp(score - largest), and target score or 0."""
+def forward(x2: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, vocab_start: int, finish: bool, z_coef: float = 0.0):
+    """Three fp32 [T]; ``finish``: logZ and loss of a whole vocabulary, and z_coef logZ^2 (None when z_coef is 0); otherwise this shard's
+    largest score, sum of exp(score - largest), and target score or 0."""
     x2, weight = _rows(x2), _rows(weight)
     (T, H), V, dev = x2.shape, weight.shape[0], x2.device
     with native.on_device(dev):
-        status = _status(dev)
-        sms = native_gemm._sms(dev)
+        status, sms = _status(dev), native_gemm._sms(dev)
         part = torch.empty((max((V + 255) // 256 * 4, 2 * sms) + 1) * T, dtype=torch.float32, device=dev)  # per part two numbers, and the target's score
-        out = torch.empty((3 if z_coef > 0 or not finish else 2, T), dtype=torch.float32, device=dev)
+        a, b = torch.empty(T, dtype=torch.float32, device=dev), torch.empty(T, dtype=torch.float32, device=dev)
+        c = torch.empty(T, dtype=torch.float32, device=dev) if z_coef > 0 or not finish else None
         native._check(native.lib().ntb_linear_ce_forward(x2.data_ptr(), x2.stride(0), weight.data_ptr(), weight.stride(0), target.data_ptr(), vocab_start, T, V, H, part.data_ptr(),
-                                                         out.data_ptr(), int(finish), z_coef, status.data_ptr(), sms, native.raw_stream(x2)), "linear_ce_forward", launches=2)
-    return out
+                                                         a.data_ptr(), b.data_ptr(), None if c is None else c.data_ptr(), finish, z_coef, status.data_ptr(), sms, native.raw_stream(x2)),
+                      "linear_ce_forward", launches=2)
+    return a, b, c
 
 
 def piece_width(T: int, V: int) -> int:
@@ -75,28 +77,37 @@ def piece_width(T: int, V: int) -> int:
     return ((V + pieces - 1) // pieces + 255) // 256 * 256
 
 
+@lru_cache(maxsize=64)
+def _backward_plan(T: int, V: int, H: int, sms: int, need_dx: bool, piece_elements: int, piece_min: int):
+    """(piece width, pitch of d, chunks of the dx product, words of scratch, word offsets of its parts or None).  Parts, each on a
+    1024-byte boundary: d (bf16 [T, pitch]), coefficients (2 T + 1), dx over several pieces (fp32 [T, H]), partial sums of a dx that is cut
+    along the vocabulary."""
+    width = piece_width(T, V)
+    pitch = (min(width, V) + 63) // 64 * 64
+    split = native.lib().ntb_linear_ce_dx_split(T, min(width, V), H, sms) if need_dx else 1
+    parts = [T * pitch // 2, 2 * T + 1, T * H if need_dx and width < V else 0, split * ((T + 255) // 256) * ((H + 255) // 256) * 65536 if split > 1 else 0]
+    ends = list(accumulate((n + 255) // 256 * 256 for n in parts))
+    return width, pitch, split, ends[-1], [e - (n + 255) // 256 * 256 if n else None for n, e in zip(parts, ends)]
+
+
 def backward(x2, weight, target, logz, g, gz: Optional[torch.Tensor], z_coef: float, vocab_start: int, need_dx: bool, need_dw: bool, main_grad: Optional[torch.Tensor] = None):
     """(dx, dw) in bf16 for the upstream gradients ``g`` of the losses and ``gz`` of the terms z_coef logZ^2 (fp32 [T]); with
     ``main_grad`` (fp32 [V, H]) dw is added to it and None is returned in its place."""
     x2, weight = _rows(x2), _rows(weight)
     (T, H), V, dev = x2.shape, weight.shape[0], x2.device
-    L, sms, ptr = native.lib(), native_gemm._sms(dev), native._ptr
+    sms = native_gemm._sms(dev)
+    width, pitch, split, words, offsets = _backward_plan(T, V, H, sms, need_dx, PIECE_ELEMENTS, PIECE_MIN)
     with native.on_device(dev):
-        width = piece_width(T, V)
-        pitch = (min(width, V) + 63) // 64 * 64
+        scratch = torch.empty(words, dtype=torch.float32, device=dev)
+        base = scratch.data_ptr()
+        d, rows, acc, ws = [None if at is None else base + 4 * at for at in offsets]
         dx = torch.empty((T, H), dtype=torch.bfloat16, device=dev) if need_dx else None
-        split = L.ntb_linear_ce_dx_split(T, min(width, V), H, sms) if need_dx else 1
-        # scratch, in fp32 words with every part on a 1024-byte boundary: d (bf16 [T, pitch]), coefficients (2 T + 1), dx over several
-        # pieces (fp32 [T, H]), partial sums of a dx that is cut along the vocabulary
-        parts = [T * pitch // 2, 2 * T + 1, T * H if need_dx and width < V else 0, split * ((T + 255) // 256) * ((H + 255) // 256) * 65536 if split > 1 else 0]
-        ends = list(accumulate((n + 255) // 256 * 256 for n in parts))
-        scratch = torch.empty(ends[-1], dtype=torch.float32, device=dev)
-        d, rows, acc, ws = (scratch.data_ptr() + 4 * (e - (n + 255) // 256 * 256) if n else None for n, e in zip(parts, ends))
         dw = torch.empty((V, H), dtype=torch.bfloat16, device=dev) if need_dw and main_grad is None else None
-        into = (main_grad if main_grad is not None else dw) if need_dw else None
+        into = (dw if main_grad is None else main_grad) if need_dw else None
+        rc = native.lib().ntb_linear_ce_backward(
+            x2.data_ptr(), x2.stride(0), weight.data_ptr(), weight.stride(0), target.data_ptr(), vocab_start, logz.data_ptr(), g.data_ptr(), None if gz is None else gz.data_ptr(), z_coef,
+            T, V, H, width, d, pitch, rows, None if dx is None else dx.data_ptr(), acc, split, ws, None if into is None else into.data_ptr(), H if into is None else into.stride(0),
+            main_grad is not None, _status(dev).data_ptr(), sms, native.raw_stream(x2))
         pieces = (V + width - 1) // width
-        rc = L.ntb_linear_ce_backward(x2.data_ptr(), x2.stride(0), weight.data_ptr(), weight.stride(0), target.data_ptr(), vocab_start, logz.data_ptr(), g.data_ptr(), ptr(gz), z_coef,
-                                      T, V, H, width, d, pitch, rows, ptr(dx), acc, split, ws, ptr(into), into.stride(0) if need_dw else H,
-                                      int(main_grad is not None), _status(dev).data_ptr(), sms, native.raw_stream(x2))
         native._check(rc, "linear_ce_backward", launches=1 + pieces * (1 + (1 + (split > 1)) * need_dx + need_dw) + (acc is not None))
     return dx, dw

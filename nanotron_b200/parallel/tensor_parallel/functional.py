@@ -286,7 +286,8 @@ def _linear_cross_entropy_forward(x, weight, target, group, z_loss_coef: float):
     tp = group.size() if group is not None else 1
     rank = dist.get_rank(group) if tp > 1 else 0
     lead = x.shape[:-1]
-    x2, tgt = x.reshape(-1, x.shape[-1]), target.reshape(-1).to(torch.int64).contiguous()
+    x2 = x if len(lead) == 1 else x.reshape(-1, x.shape[-1])
+    tgt = target.reshape(-1).to(torch.int64).contiguous()
     vocab_start = rank * weight.shape[0]
     z = None
     if x2.shape[0] == 0:
@@ -307,7 +308,9 @@ def _linear_cross_entropy_forward(x, weight, target, group, z_loss_coef: float):
             loss = logz - packed[1]
     if z is None and z_loss_coef > 0:
         z = z_loss_coef * logz.square()
-    return loss.view(lead), (z.view(lead) if z is not None else None), x2, tgt, logz, vocab_start
+    if len(lead) != 1:
+        loss, z = loss.view(lead), (z.view(lead) if z is not None else None)
+    return loss, z, x2, tgt, logz, vocab_start
 
 
 class _LinearCrossEntropy(torch.autograd.Function):
