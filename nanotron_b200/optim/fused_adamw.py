@@ -202,7 +202,7 @@ class FusedAdamW(torch.optim.Optimizer):
                     continue
                 st = self._init_state(p)
                 st["step"] += 1
-                calls.setdefault((group["betas"], group["eps"], float(st["step"])), []).append((p, st, float(group["lr"]), float(group["weight_decay"])))
+                calls.setdefault((tuple(group["betas"]), group["eps"], float(st["step"])), []).append((p, st, float(group["lr"]), float(group["weight_decay"])))
         scale = self.grad_scale.to(torch.float32) if self.grad_scale is not None else None
         for (betas, eps, step), items in calls.items():
             ps = [p for p, *_ in items]

@@ -95,6 +95,17 @@ def test_no_tokens_frozen_operands_and_main_grad():
     assert z is None and loss.shape == (6,)
 
 
+def test_one_token_and_leading_dimensions():
+    x, w, y, _ = inputs(6, 8, 20, "cpu", torch.float32)
+    want = linear_cross_entropy(x, w, y)
+    assert torch.equal(linear_cross_entropy(x.view(2, 3, 8), w, y.view(2, 3)), want.view(2, 3))
+    one = x[4].clone().requires_grad_()
+    loss = linear_cross_entropy(one, w, y[4])
+    loss.backward()
+    assert loss.shape == () and one.grad.shape == (8,)
+    torch.testing.assert_close(loss, want[4])
+
+
 def test_refusals():
     x, w, y, _ = inputs(6, 8, 20, "cpu", torch.float32)
     for bad in [(x[:, :7], w, y), (x, w[0], y), (x, w.double(), y), (x, w, y[:5]), (x, w, y.float()), (x, w[:0], y), (x.long(), w.long(), y)]:
@@ -280,6 +291,70 @@ def test_captured_step_replays_on_new_inputs():
     torch.cuda.synchronize()
     for *_, out in graphs:
         assert all(torch.equal(p, q) for p, q in zip(out, want))
+
+
+@gpu
+def test_backward_can_be_repeated():
+    x, w, y, g = inputs(70, 128, 900, DEV, torch.bfloat16)
+    a, b = x.requires_grad_(), w.requires_grad_()
+    loss, z = linear_cross_entropy_with_z_loss(a, b, y, z_loss_coef=1e-3)
+    first = torch.autograd.grad((loss, z), (a, b), (g, g), retain_graph=True)
+    second = torch.autograd.grad((loss, z), (a, b), (g, g))
+    assert all(torch.equal(p, q) for p, q in zip(first, second))
+    only_z = torch.autograd.grad(linear_cross_entropy_with_z_loss(a, b, y, z_loss_coef=1e-3)[1], a, g)  # the loss itself unused
+    assert only_z[0].isfinite().all()
+
+
+FRESH = """
+import sys
+sys.path[:0] = [{root!r}, {root!r} + "/tests"]
+import torch
+from nanotron_b200.parallel.tensor_parallel.functional import linear_cross_entropy
+from test_linear_cross_entropy import inputs
+x, w, y, g = inputs(20, 64, 300, "cuda", torch.bfloat16)
+linear_cross_entropy(x, w, y)
+torch.cuda.synchronize()
+def step():
+    a, b = x.detach().requires_grad_(), w.detach().requires_grad_()
+    loss = linear_cross_entropy(a, b, y)
+    return (loss.detach(),) + torch.autograd.grad(loss, (a, b), g)
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    out = step()
+graph.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(p, q) for p, q in zip(out, step()))
+print("captured")
+"""
+
+
+@gpu
+def test_first_backward_of_a_process_inside_a_capture():
+    """The autograd thread meets the library for the first time while the stream is being captured."""
+    import os
+    import subprocess
+    import sys
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", FRESH.format(root=root)], capture_output=True, text=True, timeout=200)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stderr[-2000:]
+
+
+@gpu
+def test_first_call_inside_a_capture_is_refused():
+    from nanotron_b200.ops import native, native_gemm
+
+    x, w, y, _ = inputs(20, 64, 300, DEV, torch.bfloat16)
+    linear_cross_entropy(x, w, y)
+    known = native_gemm._STATUS.pop(str(x.device))
+    try:
+        with pytest.raises(native.NativeKernelError, match="captured"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                linear_cross_entropy(x, w, y)
+    finally:
+        native_gemm._STATUS[str(x.device)] = known
+    torch.cuda.synchronize()
+    linear_cross_entropy(x, w, y)
 
 
 @gpu
