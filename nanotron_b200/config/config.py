@@ -490,7 +490,7 @@ def _declared_model_config_class(config_class: Type) -> Optional[Type]:
         return None
 
 
-_LEGACY_ADAM_KEYS = ("adam_beta1", "adam_beta2", "adam_eps", "torch_adam_is_fused")
+_LEGACY_ADAM_KEYS = ("adam_beta1", "adam_beta2", "adam_eps", "torch_adam_is_fused", "state_bits")
 
 
 def upgrade_legacy_config_dict(config_dict: dict) -> dict:
