@@ -222,8 +222,8 @@ __device__ __forceinline__ void p_ce_gradient(uint32_t (&r)[32], int valid, int 
   }
 }
 
-// EW: epilogue warps per CTA, 4 (each takes 32 rows), or with P_OUT_CE_STATS, which stages nothing in shared memory, 8 (each takes 32
-// rows and half of the columns).
+// EW: epilogue warps per CTA, 4 (each takes 32 rows), or in the cross entropy modes 8 (each takes 32 rows and half of the columns; where
+// the epilogue stages its output, P_OUT_CE_GRAD, the staging of the other four takes the memory of one operand stage).
 template <bool A_MN, bool B_MN, int OUT, int P_STAGES, class EXT = PPlain, int EW = P_EPI_WARPS>
 __global__ void __launch_bounds__(32 * (2 + EW), 1)
 gemm2_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b, const __grid_constant__ CUtensorMap tmap_d,
@@ -233,7 +233,7 @@ gemm2_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   constexpr int EPI_BYTES = OUT == P_OUT_CE_STATS ? 0 : EW * 2 * P_EPI_BUF;
-  static_assert(P_STAGES * P_STAGE_BYTES + EPI_BYTES + 1024 + 512 <= P_SMEM && P_STAGES <= P_MAX_STAGES && (EW == 4 || (EW == 8 && OUT == P_OUT_CE_STATS)), "shared memory of a launch");
+  static_assert(P_STAGES * P_STAGE_BYTES + EPI_BYTES + 1024 + 512 <= P_SMEM && P_STAGES <= P_MAX_STAGES && (EW == 4 || (EW == 8 && (OUT == P_OUT_CE_STATS || OUT == P_OUT_CE_GRAD))), "shared memory of a launch");
   uint8_t* epi_smem = smem + P_STAGES * P_STAGE_BYTES;
   uint64_t* bars = reinterpret_cast<uint64_t*>(epi_smem + EPI_BYTES);
   uint64_t* full_bar = bars;                       // [STAGES]  (leader) both CTAs' loads of the stage have landed
@@ -381,6 +381,7 @@ gemm2_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
   } else {
     // ------------------------------------------------------------------ epilogue warps (both CTAs, own 128 rows)
     const int q = warp & 3;
+    const int half = EW == 8 ? (warp - 2) >> 2 : 0;  // of the columns
     uint8_t* my_epi = epi_smem + (warp - 2) * 2 * P_EPI_BUF;
     constexpr bool BF16_OUT = (OUT == P_OUT_BF16 || OUT == P_OUT_PEER_BF16 || OUT == P_OUT_CE_GRAD);
     float alpha = 1.f;
@@ -415,9 +416,8 @@ gemm2_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
         }
         float m = -INFINITY, s = 0.f;
         constexpr int PARTS = EW / 4, PART_CHUNKS = P_BLOCK_N / 32 / PARTS;
-        const int part = (warp - 2) >> 2;
 #pragma unroll 1
-        for (int c = part * PART_CHUNKS; c < (part + 1) * PART_CHUNKS && c * 32 < cols; c++) {
+        for (int c = half * PART_CHUNKS; c < (half + 1) * PART_CHUNKS && c * 32 < cols; c++) {
           uint32_t r0[32];
           ptx::tmem_ld_32x32(taddr + c * 32, r0);
           ptx::tmem_ld_wait();
@@ -429,7 +429,7 @@ gemm2_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
               if (j == tj) ext.tgt[row] = __uint_as_float(r0[j]);
           }
         }
-        if (row < M) ext.part[static_cast<int64_t>(tc.n_blk * PARTS + part) * M + row] = make_float2(m, s);
+        if (row < M) ext.part[static_cast<int64_t>(tc.n_blk * PARTS + half) * M + row] = make_float2(m, s);
       } else {
       float ce_lz = 0.f, ce_coef = 0.f, ce_g = 0.f;
       int ce_t = -1, ce_cols = 0;
@@ -445,7 +445,7 @@ gemm2_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
         }
       }
 #pragma unroll 1
-      for (int c = 0; c < CHUNKS; c++) {
+      for (int c = EW == 8 ? half * (CHUNKS / 2) : 0; c < (EW == 8 ? (half + 1) * (CHUNKS / 2) : CHUNKS); c++) {
         uint8_t* stage_buf = my_epi + buf * P_EPI_BUF;
         if (lane == 0) ptx::tma_wait_group_read<1>();
         __syncwarp();

@@ -329,16 +329,17 @@ int ce_band(int M, int K) {
   return band > tiles_m ? tiles_m : band;
 }
 
-// The statistics' epilogue is the longest (an exponential per score and nothing to store) and the only one that needs no shared memory:
-// eight warps share it (2048 x 256 x 32000: 60 -> 51 us, 2047 x 768 x 50257: 115 -> 109 us; level at H = 4096).  The gradient's with
-// eight warps and one operand stage less measured level (2047 x 768 x 50257: 337 us for the three products against 334) and keeps four.
-constexpr int CE_STATS_WARPS = 8;
+// The epilogues that take an exponential per score get eight warps; with a short product four of them are what a tile waits for.  Four |
+// eight warps, us: statistics of 2048 x 256 x 32000 60 | 51, 2047 x 768 x 50257 115 | 109; gradient (one operand stage less) 72 | 59, 127 |
+// 123; level from H = 1024 on.  The plain products' epilogues gain nothing and keep four.
+constexpr int CE_WARPS = 8;
 
 template <bool A_MN, bool B_MN, int OUT, class EXT>
 int ce_launch(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& td, int M, int N, int K, const PSched& sched, const CUtensorMap& tws, const EXT& ext,
               int* status, int num_sms, cudaStream_t stream) {
-  constexpr int EW = OUT == P_OUT_CE_STATS ? CE_STATS_WARPS : P_EPI_WARPS;
-  auto kern = gemm2_tcgen05_kernel<A_MN, B_MN, OUT, P_MAX_STAGES, EXT, EW>;
+  constexpr int EW = OUT == P_OUT_CE_STATS || OUT == P_OUT_CE_GRAD ? CE_WARPS : P_EPI_WARPS;
+  constexpr int STAGES = OUT == P_OUT_CE_GRAD ? P_MAX_STAGES - 1 : P_MAX_STAGES;
+  auto kern = gemm2_tcgen05_kernel<A_MN, B_MN, OUT, STAGES, EXT, EW>;
   static bool done[64] = {};
   if (int rc = ce_configure(kern, done, P_SMEM)) return rc;
   static const PPeerMaps no_maps = {};
@@ -547,7 +548,7 @@ NTB_EXPORT int ntb_linear_ce_forward(const void* x, int64_t ldx, const void* w, 
       !p_get_encode())
     return NTB_ERR_ARG;
   // partial statistics per token: one of every half tile (the last may have no columns: (-inf, 0)), or one of every CTA
-  const int tiles = ce_few_groups(T, H) ? few_grid(V, num_sms) : (V + P_BLOCK_N - 1) / P_BLOCK_N * (CE_STATS_WARPS / 4);
+  const int tiles = ce_few_groups(T, H) ? few_grid(V, num_sms) : (V + P_BLOCK_N - 1) / P_BLOCK_N * (CE_WARPS / 4);
   float* tgt = part + static_cast<int64_t>(tiles) * 2 * T;
   const int rc = ce_stats(x, ldx, w, ldw, target, vocab_start, T, V, H, part, tgt, status, num_sms, stream);
   if (rc != NTB_OK) return rc;
