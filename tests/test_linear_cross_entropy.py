@@ -218,6 +218,22 @@ def test_main_grad_takes_the_gradient_in_one_piece():
 
 
 @gpu
+@pytest.mark.parametrize("T", [5, 300])
+def test_frozen_operands_get_no_gradient_and_cost_none(T):
+    x, w, y, g = inputs(T, 128, 999, DEV, torch.bfloat16)
+    _, _, p, d, dx, dw = definition(x, w, y, g)
+    bl, bx, bw = bounds(x, w, p, d, dx, dw, torch.zeros(T, device=DEV))
+    a = x.detach().requires_grad_()
+    (linear_cross_entropy(a, w, y) * g).sum().backward()
+    within(a.grad, dx, bx, "dx")
+    b = w.detach().requires_grad_()
+    n0 = ops.native_launches()
+    (linear_cross_entropy(x, b, y) * g).sum().backward()
+    assert ops.native_launches() - n0 == 2 + 3  # statistics, join; coefficients, gradient of the scores, dw
+    within(b.grad, dw, bw, "dw")
+
+
+@gpu
 def test_peaked_and_masked_rows():
     """Certain tokens (one score far above the rest), targets outside the vocabulary, masked rows, all rows masked, tiny upstream."""
     x, w, y, g = inputs(70, 64, 600, DEV, torch.bfloat16, spread=1.0)
