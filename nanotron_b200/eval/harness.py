@@ -3,7 +3,8 @@
 ``LogLikelihoodScorer`` turns (prompt, continuation) pairs into summed log-probabilities of the continuation tokens: prompts and
 continuations are tokenised separately, concatenated, left-padded into batches and pushed through the model exactly as generation
 does (pipeline stages exchange activations through ``PipelineEvalBatchState``; the last stage holds the vocabulary-sharded logits,
-whose per-token cross entropy is computed without gathering the vocabulary).  ``evaluate_task`` applies the task's prompt
+whose per-token cross entropy is computed without gathering the vocabulary; under ``ops.set_loss("fused")`` the head runs for the scored
+positions only, inside the cross entropy).  ``evaluate_task`` applies the task's prompt
 formulation to every document and aggregates accuracy under the token / character / PMI normalisations.
 """
 from __future__ import annotations
@@ -15,11 +16,13 @@ import torch
 from nanotron_b200 import distributed as dist
 from nanotron_b200.eval.evaluation_tasks import EvalTask, Request, accuracy, aggregate, build_request, choice_scores
 from nanotron_b200.generation.decode import _forward_logits, _model_takes_position_ids
+from nanotron_b200.models.qwen import head_feeds_loss
 from nanotron_b200.parallel import ParallelContext
 from nanotron_b200.parallel.pipeline_parallel.context_manager import attach_pipeline_state_to_model
 from nanotron_b200.parallel.pipeline_parallel.state import PipelineEvalBatchState
 from nanotron_b200.parallel.pipeline_parallel.tensor_pointer import TensorPointer
-from nanotron_b200.parallel.tensor_parallel.functional import sharded_cross_entropy
+from nanotron_b200.parallel.tensor_parallel.functional import linear_cross_entropy, sharded_cross_entropy
+from nanotron_b200.parallel.tensor_parallel.nn import DeferredLogits
 
 
 class LogLikelihoodScorer:
@@ -69,12 +72,20 @@ class LogLikelihoodScorer:
                     mask[r, width - len(row) :] = True
                 ids, mask = ids.to(device), mask.to(device)
                 second = (mask.long().cumsum(-1) - 1).clamp_(min=0) if self.takes_pos else mask
-                logits = _forward_logits(self.model, ids if is_first else TensorPointer(0), second if is_first else TensorPointer(0), self.takes_pos)
+                with head_feeds_loss(getattr(self.model, "lm_head", None)):
+                    logits = _forward_logits(self.model, ids if is_first else TensorPointer(0), second if is_first else TensorPointer(0), self.takes_pos)
                 sums = torch.zeros(len(rows), dtype=torch.float32, device=device)
                 if is_last:
                     # position p predicts token p + 1: score the continuation tokens only
                     targets = torch.roll(ids, shifts=-1, dims=1).reshape(-1)
-                    nll = sharded_cross_entropy(logits.reshape(ids.numel(), -1), targets.contiguous(), group=ctx.tp_pg, dtype=torch.float).view(len(rows), width)
+                    if isinstance(logits, DeferredLogits):
+                        # the head has not run yet: it does so for the scored positions alone
+                        at = torch.cat([torch.arange((r + 1) * width - len(encoded[i][1]) - 1, (r + 1) * width - 1) for r, i in enumerate(idx)]).to(device)
+                        nll = torch.zeros(ids.numel(), dtype=torch.float32, device=device)
+                        nll[at] = linear_cross_entropy(logits.x.index_select(0, at), logits.weight, targets[at], group=ctx.tp_pg)
+                        nll = nll.view(len(rows), width)
+                    else:
+                        nll = sharded_cross_entropy(logits.reshape(ids.numel(), -1), targets.contiguous(), group=ctx.tp_pg, dtype=torch.float).view(len(rows), width)
                     for r, i in enumerate(idx):
                         n = len(encoded[i][1])
                         sums[r] = -nll[r, width - n - 1 : width - 1].sum()

@@ -319,11 +319,11 @@ def masked_mean(loss, label_mask, dtype):
 
 
 @contextmanager
-def head_feeds_loss(head: PipelineBlock, loss: PipelineBlock):
-    """Inside: the head may hand its operands to the loss instead of the logits (``ops.set_loss("fused")``), if this pipeline stage runs
-    both (logits that travel to another stage have to exist)."""
+def head_feeds_loss(head: PipelineBlock, loss: Optional[PipelineBlock] = None):
+    """Inside: the head may hand its operands to the loss (or to a caller that takes ``DeferredLogits``) instead of the logits, under
+    ``ops.set_loss("fused")`` and if this pipeline stage runs both (logits that travel to another stage have to exist)."""
     block = getattr(head, "pp_block", None)
-    if block is None or head.rank != loss.rank:
+    if block is None or (loss is not None and head.rank != loss.rank):
         yield
         return
     block.feeds_loss = True

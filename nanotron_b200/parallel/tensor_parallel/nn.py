@@ -59,13 +59,13 @@ class TensorParallelColumnLinear(nn.Linear):
         super().__init__(in_features=self.in_features, out_features=self.out_features, bias=bias, device=device, dtype=dtype)
         self.mode = mode
         self.async_communication = async_communication
-        self.feeds_loss = False  # set by a training model around its forward when this is its head and the loss runs on the same stage
+        self.feeds_loss = False  # set around a forward whose output goes straight into the loss, on this stage (models.qwen.head_feeds_loss)
         if contiguous_chunks is not None:
             assert sum(contiguous_chunks) == out_features, f"Sum of contiguous chunks ({sum(contiguous_chunks)}) must equal out_features ({out_features})"
         mark_all_parameters_in_module_as_sharded(self, pg=self.pg, split_config=SplitConfig(split_dim=0, contiguous_chunks=contiguous_chunks))
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
-        if self.feeds_loss and self.training and self.bias is None and ops.get_loss() == "fused" and ops.linear_ce_supported(x, self.weight):
+        if self.feeds_loss and self.bias is None and ops.get_loss() == "fused" and ops.linear_ce_supported(x, self.weight):
             full = differentiable_identity(x, self.pg) if self.mode is TensorParallelLinearMode.ALL_REDUCE else differentiable_all_gather(x, self.pg)
             return {"logits": DeferredLogits(full, self.weight)}  # a head's block names its output "logits"
         return column_linear(

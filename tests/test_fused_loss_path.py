@@ -51,6 +51,23 @@ def test_fused_loss_trains_like_logits_in_every_layout(tmp_path, monkeypatch):
             assert abs(a - b) < 2e-4 * b, (model, layout, got, want[model])
 
 
+def test_scoring_runs_the_head_for_the_scored_positions_alone(tmp_path, monkeypatch):
+    from test_eval_cpu import _scorer_run
+
+    def run(name, world, **layout):
+        f = str(tmp_path / f"{name}.pt")
+        run_distributed(_scorer_run, world, out_file=f, **layout)
+        return torch.load(f)
+
+    want = run("logits", 1, tp=1, pp=1)
+    monkeypatch.setenv("NTB_LOSS", "fused")
+    for world, layout in ((1, dict(tp=1, pp=1)), (4, dict(tp=2, pp=2))):
+        got = run(f"fused_{world}", world, **layout)
+        for (x, nx), (y, ny) in zip(got["ll"], want["ll"]):
+            assert nx == ny and abs(x - y) < 1e-3, (layout, got["ll"], want["ll"])
+        assert got["res"] == want["res"]
+
+
 def _trainer(model_config, loss="logits", state_bits=32, **kw):
     import nanotron_b200.config as c
     from nanotron_b200.trainer import DistributedTrainer
@@ -85,11 +102,11 @@ def test_configuration_selects_loss_and_states(default_loss):
     t.training_step(iter([batch]))
     assert len(seen) == 1 and isinstance(seen[0], DeferredLogits)
     model = t.unwrapped_model
-    model.eval()  # scoring and generation read the logits
+    model.eval()  # outside the model's own forward (generation) it gives logits
     ids = torch.zeros(1, 4, dtype=torch.long)
     assert torch.is_tensor(model.model(input_ids=ids, input_mask=torch.ones_like(ids, dtype=torch.bool)))
     model.train()
-    assert torch.is_tensor(model.model(input_ids=ids, input_mask=torch.ones_like(ids, dtype=torch.bool)))  # nor outside the model's own forward
+    assert torch.is_tensor(model.model(input_ids=ids, input_mask=torch.ones_like(ids, dtype=torch.bool)))
     states = [s for s in t.optimizer.get_base_optimizer().state.values()]
     assert states and all(s["exp_avg"].dtype == torch.uint8 for s in states)
     t.parallel_context.destroy()
