@@ -58,6 +58,12 @@ struct PCeArgs {
   const float* g = nullptr;
 };
 
+// The tensor cores cut what does not fit when they add to an accumulator: a sum over K comes out small by about 2^-26 of its value per 16
+// products (measured: 9e-10 K).  For the loss that is the largest error (4e-6 of every score at K = 4096), so its scores are accumulated
+// over at most this many k-blocks (1024 products) and the pieces added in registers, rounding to nearest: the loss is then off by 2.7e-7
+// of its value instead of 1.1e-6 (K = 4096) or 2.4e-6 (8192).  4096 x 2048 x 128256: 1265 -> 1290 us.
+constexpr int P_CE_SEGMENT = 16;
+
 constexpr float P_LOG2E = 1.4426950408889634f;
 __device__ __forceinline__ float p_ex2(float x) {
   float y;
@@ -181,25 +187,26 @@ __device__ __forceinline__ PTile pair_tile(int t, int tiles_m, int tiles_n, int 
 
 // Running (largest, sum of exponentials) of a row over 32 more scores.  One pass: when the largest grows, the sum so far is rescaled
 // once per 32 scores, not per score.  Scores are folded as 2^(score log2 e - largest log2 e): one FMA and one ex2 each.
-__device__ __forceinline__ void p_ce_accumulate(const uint32_t (&r)[32], int valid, float& m, float& s) {
+template <int W>
+__device__ __forceinline__ void p_ce_accumulate(const uint32_t (&r)[W], int valid, float& m, float& s) {
   float cm = -INFINITY;
-  if (valid >= 32) {
+  if (valid >= W) {
 #pragma unroll
-    for (int j = 0; j < 32; j++) cm = fmaxf(cm, __uint_as_float(r[j]));
+    for (int j = 0; j < W; j++) cm = fmaxf(cm, __uint_as_float(r[j]));
   } else {
 #pragma unroll
-    for (int j = 0; j < 32; j++)
+    for (int j = 0; j < W; j++)
       if (j < valid) cm = fmaxf(cm, __uint_as_float(r[j]));
   }
   const float nm = fmaxf(m, cm);
   const float base = nm == -INFINITY ? 0.f : nm * P_LOG2E;  // a row of -inf scores keeps the sum 0 instead of inf - inf
   float a[4] = {0.f, 0.f, 0.f, 0.f};
-  if (valid >= 32) {
+  if (valid >= W) {
 #pragma unroll
-    for (int j = 0; j < 32; j++) a[j & 3] += p_ex2(fmaf(__uint_as_float(r[j]), P_LOG2E, -base));
+    for (int j = 0; j < W; j++) a[j & 3] += p_ex2(fmaf(__uint_as_float(r[j]), P_LOG2E, -base));
   } else {
 #pragma unroll
-    for (int j = 0; j < 32; j++)
+    for (int j = 0; j < W; j++)
       if (j < valid) a[j & 3] += p_ex2(fmaf(__uint_as_float(r[j]), P_LOG2E, -base));
   }
   s = s * p_ex2(fmaf(m, P_LOG2E, -base)) + ((a[0] + a[1]) + (a[2] + a[3]));
@@ -222,10 +229,19 @@ __device__ __forceinline__ void p_ce_gradient(uint32_t (&r)[32], int valid, int 
   }
 }
 
+// P_OUT_CE_STATS keeps 128 scores of a row in every epilogue thread.  Its warps come in groups of four that exchange registers: the
+// first group (producer, MMA issuer, two idle warps) hands most of its own to the two epilogue groups.  The shares add up to what the
+// block is launched with (168 x 384); the host checks that before the launch.  (Without the exchange the scores spill, 168 registers at
+// eight or 96 at sixteen epilogue warps, and the pass takes 1.3 times as long.)
+constexpr int P_SPLIT_REGS = 168, P_SPLIT_REGS_LOAD = 72, P_SPLIT_REGS_EPI = 216;
+static_assert(4 * P_SPLIT_REGS_LOAD + 8 * P_SPLIT_REGS_EPI == 12 * P_SPLIT_REGS, "register shares of the warp groups");
+constexpr int p_first_epilogue_warp(int out) { return out == P_OUT_CE_STATS ? 4 : 2; }
+constexpr int p_threads(int out, int ew) { return 32 * (p_first_epilogue_warp(out) + ew); }
+
 // EW: epilogue warps per CTA, 4 (each takes 32 rows), or in the cross entropy modes 8 (each takes 32 rows and half of the columns; where
 // the epilogue stages its output, P_OUT_CE_GRAD, the staging of the other four takes the memory of one operand stage).
 template <bool A_MN, bool B_MN, int OUT, int P_STAGES, class EXT = PPlain, int EW = P_EPI_WARPS>
-__global__ void __launch_bounds__(32 * (2 + EW), 1)
+__global__ void __launch_bounds__(p_threads(OUT, EW), 1)
 gemm2_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b, const __grid_constant__ CUtensorMap tmap_d,
                      int M, int N, int K, int band, int* __restrict__ status, const __grid_constant__ PFuse fuse, const __grid_constant__ PPeerMaps pmaps,
                      const __grid_constant__ PSched sched, const __grid_constant__ CUtensorMap tmap_ws, const __grid_constant__ CUtensorMap tmap_al,
@@ -243,6 +259,7 @@ gemm2_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
   uint32_t* tmem_base_slot = reinterpret_cast<uint32_t*>(tmem_empty + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_base_slot + 1);
 
+  constexpr int EPI0 = p_first_epilogue_warp(OUT);
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   const uint32_t cta = cluster_ctarank();  // 0 = leader
@@ -277,6 +294,8 @@ gemm2_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
   ptx::tc_fence_after();
   const uint32_t tmem_base = *tmem_base_slot;
 
+  if (warp < EPI0) {
+  if constexpr (OUT == P_OUT_CE_STATS) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(P_SPLIT_REGS_LOAD));
   if (warp == 0) {
     // ------------------------------------------------------------------ TMA producer (both CTAs)
     if (ptx::elect_one()) {
@@ -353,13 +372,16 @@ gemm2_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
         for (int u = pair; u < sched.total_units && ok; u += num_pairs) {
           const PUnit un = decode_unit(u, sched, k_blocks);
           if (un.kbs <= 0) continue;
+          int kb = 0;
+          do {  // one accumulator per tile; P_OUT_CE_STATS: one per P_CE_SEGMENT k-blocks of a tile
+          const int kb0 = kb, kb1 = OUT == P_OUT_CE_STATS ? min(kb + P_CE_SEGMENT, un.kbs) : un.kbs;
           const int acc = tile_it & 1;
           const uint32_t acc_ph = (tile_it >> 1) & 1;
           tile_it++;
           if (!ptx::mbar_wait(&tmem_empty[acc], acc_ph ^ 1, abort_flag)) { ok = false; break; }
           ptx::tc_fence_after();
           const uint32_t tmem_d = tmem_base + acc * P_BLOCK_N;
-          for (int kb = 0; kb < un.kbs; kb++, it++) {
+          for (; kb < kb1; kb++, it++) {
             const int s = it % P_STAGES;
             const uint32_t ph = (it / P_STAGES) & 1;
             if (!ptx::mbar_wait(&full_bar[s], ph, abort_flag)) { ok = false; break; }
@@ -370,19 +392,23 @@ gemm2_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
             for (int k = 0; k < P_BLOCK_K / P_UMMA_K; k++) {
               const uint64_t adesc = A_MN ? ptx::make_smem_desc(sa + k * P_UMMA_K * 128, P_BLOCK_K * 128, 1024) : ptx::make_smem_desc(sa + k * P_UMMA_K * 2, 16, 1024);
               const uint64_t bdesc = B_MN ? ptx::make_smem_desc(sb + k * P_UMMA_K * 128, P_BLOCK_K * 128, 1024) : ptx::make_smem_desc(sb + k * P_UMMA_K * 2, 16, 1024);
-              umma2_f16(tmem_d, adesc, bdesc, idesc, (kb | k) != 0 ? 1u : 0u);
+              umma2_f16(tmem_d, adesc, bdesc, idesc, ((kb - kb0) | k) != 0 ? 1u : 0u);
             }
             umma2_commit(ptx::smem_u32(&empty_bar[s]));  // the stage is free once these MMAs (in both SMs) have read it
           }
           if (ok) umma2_commit(ptx::smem_u32(&tmem_full[acc]));
+          } while (OUT == P_OUT_CE_STATS && ok && kb < un.kbs);
         }
       }
     }
+  }
   } else {
+    if constexpr (OUT == P_OUT_CE_STATS) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(P_SPLIT_REGS_EPI));
     // ------------------------------------------------------------------ epilogue warps (both CTAs, own 128 rows)
+    constexpr uint32_t POLL_NS = OUT == P_OUT_CE_STATS ? 100 : 1000;  // pieces of a tile follow one another in 4 us
     const int q = warp & 3;
-    const int half = EW == 8 ? (warp - 2) >> 2 : 0;  // of the columns
-    uint8_t* my_epi = epi_smem + (warp - 2) * 2 * P_EPI_BUF;
+    const int half = EW == 8 ? (warp - EPI0) >> 2 : 0;  // of the columns
+    uint8_t* my_epi = epi_smem + (warp - EPI0) * 2 * P_EPI_BUF;
     constexpr bool BF16_OUT = (OUT == P_OUT_BF16 || OUT == P_OUT_PEER_BF16 || OUT == P_OUT_CE_GRAD);
     float alpha = 1.f;
     if constexpr (std::is_same_v<EXT, PAlpha>) alpha = ext.alpha ? *ext.alpha : 1.f;
@@ -401,8 +427,8 @@ gemm2_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
       const bool bf16_path = BF16_OUT && !to_ws;
       const int CHUNK_COLS = bf16_path ? 64 : 32;
       const int CHUNKS = P_BLOCK_N / CHUNK_COLS;
-      if (!ptx::mbar_wait(&tmem_full[acc], acc_ph, abort_flag, 1000)) { ok = false; break; }
-      if (cta == 0 && warp == 2 && lane == 0) mbar_arrive_cluster(map_to_cta(ptx::smem_u32(&tmem_full[acc]), 1));  // forward to the peer's epilogue
+      if (!ptx::mbar_wait(&tmem_full[acc], acc_ph, abort_flag, POLL_NS)) { ok = false; break; }
+      if (cta == 0 && warp == EPI0 && lane == 0) mbar_arrive_cluster(map_to_cta(ptx::smem_u32(&tmem_full[acc]), 1));  // forward to the peer's epilogue
       ptx::tc_fence_after();
       const uint32_t taddr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * P_BLOCK_N;
       const int row0 = (tc.m_blk * 2 + static_cast<int>(cta)) * P_BLOCK_M + q * 32;
@@ -414,19 +440,67 @@ gemm2_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
           const int64_t rel = ext.target[row] - ext.col0 - static_cast<int64_t>(tc.n_blk) * P_BLOCK_N;
           if (rel >= 0 && rel < cols) t = static_cast<int>(rel);
         }
+        constexpr int PARTS = EW / 4, PART_COLS = P_BLOCK_N / PARTS;
+        const int c0 = half * PART_COLS;  // this warp's columns
         float m = -INFINITY, s = 0.f;
-        constexpr int PARTS = EW / 4, PART_CHUNKS = P_BLOCK_N / 32 / PARTS;
+        auto hand_back = [&](int a) {  // to the leader's MMA thread (a remote arrive from the peer CTA)
+          ptx::tc_fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            if (cta == 0) ptx::mbar_arrive(&tmem_empty[a]);
+            else mbar_arrive_cluster(map_to_cta(ptx::smem_u32(&tmem_empty[a]), 0));
+          }
+        };
+        if (un.kbs <= P_CE_SEGMENT) {
 #pragma unroll 1
-        for (int c = half * PART_CHUNKS; c < (half + 1) * PART_CHUNKS && c * 32 < cols; c++) {
-          uint32_t r0[32];
-          ptx::tmem_ld_32x32(taddr + c * 32, r0);
-          ptx::tmem_ld_wait();
-          p_ce_accumulate(r0, cols - c * 32, m, s);
-          const int tj = t - c * 32;
-          if (__any_sync(0xffffffffu, tj >= 0 && tj < 32)) {  // rare: 32 rows against a whole vocabulary
+          for (int c = c0; c < c0 + PART_COLS && c < cols; c += 32) {
+            uint32_t r0[32];
+            ptx::tmem_ld_32x32(taddr + c, r0);
+            ptx::tmem_ld_wait();
+            p_ce_accumulate(r0, cols - c, m, s);
+            const int tj = t - c;
+            if (__any_sync(0xffffffffu, tj >= 0 && tj < 32)) {  // rare: 32 rows against a whole vocabulary
 #pragma unroll
-            for (int j = 0; j < 32; j++)
-              if (j == tj) ext.tgt[row] = __uint_as_float(r0[j]);
+              for (int j = 0; j < 32; j++)
+                if (j == tj) ext.tgt[row] = __uint_as_float(r0[j]);
+            }
+          }
+          hand_back(acc);
+        } else {
+          // several accumulators: their sum is built in registers, eight columns at a time, and each goes back as soon as it is read
+          uint32_t sums[PART_COLS / 8][8];
+          int a = acc;
+          for (int kb = P_CE_SEGMENT;; kb += P_CE_SEGMENT) {
+            const uint32_t ta = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + a * P_BLOCK_N + c0;
+            const bool first = kb == P_CE_SEGMENT;
+#pragma unroll
+            for (int c = 0; c < PART_COLS / 8; c++) {
+              uint32_t r0[8];
+              ptx::tmem_ld_32x8(ta + c * 8, r0);
+              ptx::tmem_ld_wait();
+#pragma unroll
+              for (int j = 0; j < 8; j++) sums[c][j] = first ? r0[j] : __float_as_uint(__uint_as_float(sums[c][j]) + __uint_as_float(r0[j]));
+            }
+            hand_back(a);
+            if (kb >= un.kbs) break;
+            a = tile_it & 1;
+            if (!ptx::mbar_wait(&tmem_full[a], (tile_it >> 1) & 1, abort_flag, POLL_NS)) { ok = false; break; }
+            tile_it++;
+            if (cta == 0 && warp == EPI0 && lane == 0) mbar_arrive_cluster(map_to_cta(ptx::smem_u32(&tmem_full[a]), 1));
+            ptx::tc_fence_after();
+          }
+          if (!ok) break;
+#pragma unroll
+          for (int c = 0; c < PART_COLS / 8; c++) {
+            if (c0 + c * 8 < cols) {
+              p_ce_accumulate(sums[c], cols - c0 - c * 8, m, s);
+              const int tj = t - c0 - c * 8;
+              if (__any_sync(0xffffffffu, tj >= 0 && tj < 8)) {
+#pragma unroll
+                for (int j = 0; j < 8; j++)
+                  if (j == tj) ext.tgt[row] = __uint_as_float(sums[c][j]);
+              }
+            }
           }
         }
         if (row < M) ext.part[static_cast<int64_t>(tc.n_blk * PARTS + half) * M + row] = make_float2(m, s);
@@ -514,12 +588,14 @@ gemm2_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
         buf ^= 1;
       }
       }
-      // accumulator fully read: hand it back to the leader's MMA thread (a remote arrive from the peer CTA)
-      ptx::tc_fence_before();
-      __syncwarp();
-      if (lane == 0) {
-        if (cta == 0) ptx::mbar_arrive(&tmem_empty[acc]);
-        else mbar_arrive_cluster(map_to_cta(ptx::smem_u32(&tmem_empty[acc]), 0));
+      if constexpr (OUT != P_OUT_CE_STATS) {
+        // accumulator fully read: hand it back to the leader's MMA thread (a remote arrive from the peer CTA)
+        ptx::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          if (cta == 0) ptx::mbar_arrive(&tmem_empty[acc]);
+          else mbar_arrive_cluster(map_to_cta(ptx::smem_u32(&tmem_empty[acc]), 0));
+        }
       }
     }
     if (lane == 0) {

@@ -5,10 +5,9 @@
 //
 // Forward: one GEMM over the whole vocabulary on CTA pairs (gemm2_core.cuh) whose epilogue keeps, per token and 256-column tile, only
 // (largest score, sum of exponentials); a small kernel joins the half tiles of a token.  Scores never leave the tensor memory, and they
-// are used in fp32 (logits written in bf16 are off by up to 2^-8 of their value, several percent of a probability).  What is left is the
-// tensor cores' own rounding: they cut when they add to an accumulator, so a score comes out small by 9e-10 H of its value (4e-6 at
-// H = 4096, where the loss is off by 1e-6 of itself).  Adding pieces of 1024 products in registers instead takes that to 3e-7 at any H
-// and costs a third of the forward pass (the pieces do not fit the registers of an epilogue): not done.
+// are used in fp32 (logits written in bf16 are off by up to 2^-8 of their value, several percent of a probability).  They are accumulated
+// 1024 products at a time and the pieces added in registers, because the tensor cores cut when they add to an accumulator: the loss is
+// within 3e-7 of its value at any H (in one accumulator 1.1e-6 at H = 4096, 2.4e-6 at 8192) for 1 .. 2 % of the forward pass.
 // Backward: the vocabulary is cut into pieces; for each piece the scores are computed again, the epilogue turns them into d (bf16,
 // one rounding), and two plain products take d to dx (summed over the pieces in fp32) and to the piece's rows of dw.  Only one
 // piece of d is alive.  d is kept in units of the largest |g| (`ce_row_coefficients`) and the products are scaled back by that one
@@ -342,12 +341,21 @@ int ce_launch(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& t
   auto kern = gemm2_tcgen05_kernel<A_MN, B_MN, OUT, STAGES, EXT, EW>;
   static bool done[64] = {};
   if (int rc = ce_configure(kern, done, P_SMEM)) return rc;
+  if (OUT == P_OUT_CE_STATS) {  // its warp groups exchange registers: the block has to be launched with as many as they share out
+    static int regs = -1;
+    if (regs < 0) {
+      cudaFuncAttributes fa;
+      if (cudaFuncGetAttributes(&fa, kern) != cudaSuccess) return NTB_ERR_LAUNCH;
+      regs = fa.numRegs;
+    }
+    if (regs < P_SPLIT_REGS) return NTB_ERR_LAUNCH;
+  }
   static const PPeerMaps no_maps = {};
   int pairs = num_sms / 2;
   if (sched.total_units < pairs) pairs = sched.total_units;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(2 * pairs), 1, 1);
-  cfg.blockDim = dim3(32 * (2 + EW), 1, 1);
+  cfg.blockDim = dim3(p_threads(OUT, EW), 1, 1);
   cfg.dynamicSmemBytes = P_SMEM;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];

@@ -339,7 +339,7 @@ class _LinearCrossEntropy(torch.autograd.Function):
         return (dx.view(ctx.shape) if need_dx else None), dw, None, None, None
 
 
-def _check_linear_cross_entropy(x, weight, target, group):
+def _check_linear_cross_entropy(x, weight, target):
     if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1]:
         raise ValueError(f"hidden states [..., H] and weight [V, H] expected, got {tuple(x.shape)} and {tuple(weight.shape)}")
     if x.dtype != weight.dtype or not x.is_floating_point():
@@ -363,7 +363,7 @@ def linear_cross_entropy(x, weight, target, group: Optional[dist.ProcessGroup] =
 
 def linear_cross_entropy_with_z_loss(x, weight, target, group: Optional[dist.ProcessGroup] = None, z_loss_coef: float = 1e-4):
     """``linear_cross_entropy`` and the per-token term ``z_loss_coef * logZ^2`` (None when the coefficient is 0)."""
-    _check_linear_cross_entropy(x, weight, target, group)
+    _check_linear_cross_entropy(x, weight, target)
     if z_loss_coef < 0:
         raise ValueError(f"z_loss_coef must not be negative, got {z_loss_coef}")
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
