@@ -691,7 +691,7 @@ def adamw_multi_tensor(params, grads, exp_avgs, exp_avg_sqs, *, lr, beta1: float
 
     ``params``, ``grads``: fp32 or bf16, any sizes, params contiguous.  ``lr``, ``weight_decay``: a number, or one per tensor.  ``step``: 1 for
     the first.  ``halves``: optional bf16 tensors (or None per entry) that receive the rounded parameters.  ``grad_scale``: optional fp32
-    device scalar multiplied into every gradient (a clipping coefficient).
+    device scalar multiplied into every gradient (a clipping coefficient).  No two of the tensors that are written may share memory.
 
     States: fp32 tensors of the parameters' sizes; or, with ``exp_avg_exponents`` and ``exp_avg_sq_exponents``, uint8 codes of the
     parameters' sizes with one uint8 exponent per 128 consecutive elements (all zero: a fresh state).  8-bit states are rounded

@@ -192,7 +192,7 @@ class FusedAdamW(torch.optim.Optimizer):
                 p._half_written = True
 
     def _step8(self):
-        """All tensors with the same hyper-parameters and step number in one call (on CUDA one launch)."""
+        """All tensors of a device with the same hyper-parameters and step number in one call (on CUDA one launch)."""
         from nanotron_b200 import ops
 
         calls = {}
@@ -202,9 +202,8 @@ class FusedAdamW(torch.optim.Optimizer):
                     continue
                 st = self._init_state(p)
                 st["step"] += 1
-                calls.setdefault((tuple(group["betas"]), group["eps"], float(st["step"])), []).append((p, st, float(group["lr"]), float(group["weight_decay"])))
-        scale = self.grad_scale.to(torch.float32) if self.grad_scale is not None else None
-        for (betas, eps, step), items in calls.items():
+                calls.setdefault((tuple(group["betas"]), group["eps"], float(st["step"]), p.device), []).append((p, st, float(group["lr"]), float(group["weight_decay"])))
+        for (betas, eps, step, device), items in calls.items():
             ps = [p for p, *_ in items]
             targets = [self.half_targets.get(id(p)) for p in ps]
             halves = [h if h is not None and h.dtype == torch.bfloat16 and h.is_contiguous() else None for h in targets]
@@ -212,7 +211,7 @@ class FusedAdamW(torch.optim.Optimizer):
                 ps, [p.grad for p in ps], [st["exp_avg"] for _, st, *_ in items], [st["exp_avg_sq"] for _, st, *_ in items],
                 exp_avg_exponents=[st["exp_avg_exponents"] for _, st, *_ in items], exp_avg_sq_exponents=[st["exp_avg_sq_exponents"] for _, st, *_ in items],
                 halves=halves, lr=[lr for *_, lr, _ in items], weight_decay=[wd for *_, wd in items], beta1=betas[0], beta2=betas[1], eps=eps, step=step,
-                grad_scale=scale, seed=ref.mix32((self.state_seed * 0x9E3779B9 + int(step)) & 0xFFFFFFFF),
+                grad_scale=self._scale_on(device), seed=ref.mix32((self.state_seed * 0x9E3779B9 + int(step)) & 0xFFFFFFFF),
             )
             for p, target, written in zip(ps, targets, halves):
                 if target is None:
@@ -221,13 +220,16 @@ class FusedAdamW(torch.optim.Optimizer):
                     target.copy_(p.view(-1))
                 p._half_written = True
 
+    def _scale_on(self, device):
+        return None if self.grad_scale is None else torch.as_tensor(self.grad_scale, dtype=torch.float32, device=device)
+
     def _per_tensor_step(self):
         from nanotron_b200 import ops
 
         for group in self.param_groups:
             beta1, beta2 = group["betas"]
             lr = float(group["lr"])
-            together, alone = {}, []  # step number -> tensors that the multi-tensor kernel takes; the others
+            together, alone = {}, []  # (step number, device) -> tensors that the multi-tensor kernel takes; the others
             for p in group["params"]:
                 if p.grad is None:
                     continue
@@ -235,13 +237,12 @@ class FusedAdamW(torch.optim.Optimizer):
                 st["step"] += 1
                 item = (p, p.grad, st["exp_avg"], st["exp_avg_sq"], self.half_targets.get(id(p)))
                 if p.is_cuda and ops.get_mode() != "torch" and self._multi_tensor_takes(*item):
-                    together.setdefault(float(st["step"]), []).append(item)
+                    together.setdefault((float(st["step"]), p.device), []).append(item)
                 else:
                     alone.append((float(st["step"]), item))
-            for step_val, items in together.items():
+            for (step_val, device), items in together.items():
                 ps, gs, ms, vs, halves = (list(x) for x in zip(*items))
-                scale = self.grad_scale.to(torch.float32) if self.grad_scale is not None else None
-                ops.adamw_multi_tensor(ps, gs, ms, vs, lr=lr, beta1=beta1, beta2=beta2, eps=group["eps"], weight_decay=group["weight_decay"], step=step_val, halves=halves, grad_scale=scale)
+                ops.adamw_multi_tensor(ps, gs, ms, vs, lr=lr, beta1=beta1, beta2=beta2, eps=group["eps"], weight_decay=group["weight_decay"], step=step_val, halves=halves, grad_scale=self._scale_on(device))
             scale = float(self.grad_scale) if alone and self.grad_scale is not None else 1.0
             for step_val, (p, g, m, v, h) in alone:
                 if p.dtype == torch.float32:

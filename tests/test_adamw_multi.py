@@ -292,6 +292,26 @@ def test_8_bit_first_step_is_the_32_bit_one(device):
         torch.testing.assert_close(x, y, rtol=2.0**-20, atol=1e-2 * 2.0**-19)
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("devices", [("cpu", "cpu"), pytest.param((DEV, "cpu"), marks=gpu)])
+def test_gradient_scale_of_any_kind_and_parameters_on_two_devices(bits, devices):
+    """The scale may be a number, or a scalar of another type or device than the parameters; 0.5 is exact in all of them."""
+
+    def stepped(scale, factor):
+        params = [torch.nn.Parameter((torch.arange(300.0) / 300).to(d)) for d in devices]
+        opt = FusedAdamW(params, lr=1e-2, state_bits=bits)
+        opt.grad_scale = scale
+        for p in params:
+            p.grad = torch.linspace(-1, 1, 300).to(p.device) * factor
+        opt.step()
+        return [p.detach().cpu() for p in params]
+
+    want = stepped(None, 0.5)
+    for scale in (0.5, torch.tensor(0.5), torch.tensor([0.5], dtype=torch.float64), torch.tensor(0.5, device=devices[0])):
+        for a, b in zip(stepped(scale, 1.0), want):
+            assert torch.equal(a, b)
+
+
 # ------------------------------------------------------------------------------------------------ GPU
 @gpu
 @pytest.mark.parametrize("bits", [32, 8])
