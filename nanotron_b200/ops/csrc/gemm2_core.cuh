@@ -11,7 +11,8 @@
 // Warp roles per CTA: warp 0 TMA producer (own A rows + own half of B into the CTA's own shared memory; the loads are the
 // cta_group::2 form of cp.async.bulk.tensor, whose completion bytes are counted on the LEADER's stage barrier, so the leader's MMA
 // thread waits on one barrier for both halves); warp 1: the MMA issuer in the leader, idle in the peer; warps 2..5 epilogue
-// (tcgen05.ld -> swizzled staging -> TMA store / reduce-add of the CTA's own rows).
+// (tcgen05.ld -> swizzled staging -> TMA store / reduce-add of the CTA's own rows).  Epilogues that compute take EW = 8 warps, four to
+// each half of the columns: 2..9, or 4..11 with warps 2 and 3 idle where warp groups exchange registers (P_OUT_CE_STATS).
 // Cross-CTA signals besides the loads are plain remote mbarrier arrives: the leader's producer forwards every "stage free" to the
 // peer's producer, one leader epilogue warp forwards "accumulator ready" to the peer's epilogue, and the peer's epilogue warps hand
 // accumulators back to the leader's MMA thread.  All waits are bounded; the two CTAs meet in a cluster barrier before TMEM is freed.
@@ -374,29 +375,29 @@ gemm2_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
           if (un.kbs <= 0) continue;
           int kb = 0;
           do {  // one accumulator per tile; P_OUT_CE_STATS: one per P_CE_SEGMENT k-blocks of a tile
-          const int kb0 = kb, kb1 = OUT == P_OUT_CE_STATS ? min(kb + P_CE_SEGMENT, un.kbs) : un.kbs;
-          const int acc = tile_it & 1;
-          const uint32_t acc_ph = (tile_it >> 1) & 1;
-          tile_it++;
-          if (!ptx::mbar_wait(&tmem_empty[acc], acc_ph ^ 1, abort_flag)) { ok = false; break; }
-          ptx::tc_fence_after();
-          const uint32_t tmem_d = tmem_base + acc * P_BLOCK_N;
-          for (; kb < kb1; kb++, it++) {
-            const int s = it % P_STAGES;
-            const uint32_t ph = (it / P_STAGES) & 1;
-            if (!ptx::mbar_wait(&full_bar[s], ph, abort_flag)) { ok = false; break; }
+            const int kb0 = kb, kb1 = OUT == P_OUT_CE_STATS ? min(kb + P_CE_SEGMENT, un.kbs) : un.kbs;
+            const int acc = tile_it & 1;
+            const uint32_t acc_ph = (tile_it >> 1) & 1;
+            tile_it++;
+            if (!ptx::mbar_wait(&tmem_empty[acc], acc_ph ^ 1, abort_flag)) { ok = false; break; }
             ptx::tc_fence_after();
-            const uint32_t sa = ptx::smem_u32(smem + s * P_STAGE_BYTES);
-            const uint32_t sb = sa + P_A_BYTES;
-#pragma unroll
-            for (int k = 0; k < P_BLOCK_K / P_UMMA_K; k++) {
-              const uint64_t adesc = A_MN ? ptx::make_smem_desc(sa + k * P_UMMA_K * 128, P_BLOCK_K * 128, 1024) : ptx::make_smem_desc(sa + k * P_UMMA_K * 2, 16, 1024);
-              const uint64_t bdesc = B_MN ? ptx::make_smem_desc(sb + k * P_UMMA_K * 128, P_BLOCK_K * 128, 1024) : ptx::make_smem_desc(sb + k * P_UMMA_K * 2, 16, 1024);
-              umma2_f16(tmem_d, adesc, bdesc, idesc, ((kb - kb0) | k) != 0 ? 1u : 0u);
+            const uint32_t tmem_d = tmem_base + acc * P_BLOCK_N;
+            for (; kb < kb1; kb++, it++) {
+              const int s = it % P_STAGES;
+              const uint32_t ph = (it / P_STAGES) & 1;
+              if (!ptx::mbar_wait(&full_bar[s], ph, abort_flag)) { ok = false; break; }
+              ptx::tc_fence_after();
+              const uint32_t sa = ptx::smem_u32(smem + s * P_STAGE_BYTES);
+              const uint32_t sb = sa + P_A_BYTES;
+  #pragma unroll
+              for (int k = 0; k < P_BLOCK_K / P_UMMA_K; k++) {
+                const uint64_t adesc = A_MN ? ptx::make_smem_desc(sa + k * P_UMMA_K * 128, P_BLOCK_K * 128, 1024) : ptx::make_smem_desc(sa + k * P_UMMA_K * 2, 16, 1024);
+                const uint64_t bdesc = B_MN ? ptx::make_smem_desc(sb + k * P_UMMA_K * 128, P_BLOCK_K * 128, 1024) : ptx::make_smem_desc(sb + k * P_UMMA_K * 2, 16, 1024);
+                umma2_f16(tmem_d, adesc, bdesc, idesc, ((kb - kb0) | k) != 0 ? 1u : 0u);
+              }
+              umma2_commit(ptx::smem_u32(&empty_bar[s]));  // the stage is free once these MMAs (in both SMs) have read it
             }
-            umma2_commit(ptx::smem_u32(&empty_bar[s]));  // the stage is free once these MMAs (in both SMs) have read it
-          }
-          if (ok) umma2_commit(ptx::smem_u32(&tmem_full[acc]));
+            if (ok) umma2_commit(ptx::smem_u32(&tmem_full[acc]));
           } while (OUT == P_OUT_CE_STATS && ok && kb < un.kbs);
         }
       }
