@@ -61,8 +61,9 @@ struct PCeArgs {
 
 // The tensor cores cut what does not fit when they add to an accumulator: a sum over K comes out small by about 2^-26 of its value per 16
 // products (measured: 9e-10 K).  For the loss that is the largest error (4e-6 of every score at K = 4096), so its scores are accumulated
-// over at most this many k-blocks (1024 products) and the pieces added in registers, rounding to nearest: the loss is then off by 2.7e-7
-// of its value instead of 1.1e-6 (K = 4096) or 2.4e-6 (8192).  4096 x 2048 x 128256: 1265 -> 1290 us.
+// over at most this many k-blocks (1024 products) and the pieces added in registers, rounding to nearest: the loss (of
+// scores with a standard deviation of 1.5) is then off by 2.7e-7 of its value instead of 1.1e-6 (K = 4096) or 2.4e-6 (8192).  us, one
+// accumulator -> pieces: 4096 x 2048 x 128256 1265 -> 1290, 16384 x 2048 x 128256 5650 -> 5795.
 constexpr int P_CE_SEGMENT = 16;
 
 constexpr float P_LOG2E = 1.4426950408889634f;
