@@ -50,6 +50,7 @@ struct PAlpha {
 struct PCeArgs {
   const int64_t* target = nullptr;  // [M] class of every row, in the numbering in which column 0 of this product is `col0`
   int64_t col0 = 0;
+  int a_rows = P_BLOCK_M;           // rows per load of A: P_BLOCK_M, or all there are in steps of 8
   // P_OUT_CE_STATS: nothing but these leaves the kernel
   float2* part = nullptr;           // [tiles_n * EW / 4][M] (largest score, sum exp(score - largest)) of every 1024 / EW columns
   float* tgt = nullptr;             // [M] the target's score, written where the target is one of this product's columns
@@ -72,6 +73,10 @@ __device__ __forceinline__ float p_ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+
+// In a kernel that may have been launched before the one in front of it in the stream is complete: waits until it is, and its writes are seen.
+// Returns at once after an ordinary launch.
+__device__ __forceinline__ void p_wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 // Tensor-parallel fusion on the pair kernel (same protocol as the one-CTA kernel in gemm_tcgen05.cu; all off when world == 0):
 //  * all-gather -> GEMM: A is a gathered buffer of `world` row blocks of `ag_rows` rows that peers fill with plain stores;
@@ -286,12 +291,20 @@ gemm2_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
     ptx::prefetch_tmap(&tmap_b);
     ptx::prefetch_tmap(&tmap_d);
   }
+  if constexpr (std::is_same_v<EXT, PCeArgs>) {
+    if (M <= P_BLOCK_M) {  // rows of A that no load fills
+      for (int i = threadIdx.x; i < P_STAGES * (P_A_BYTES / 16); i += blockDim.x)
+        *reinterpret_cast<uint4*>(smem + (i / (P_A_BYTES / 16)) * P_STAGE_BYTES + (i % (P_A_BYTES / 16)) * 16) = make_uint4(0, 0, 0, 0);
+      ptx::fence_proxy_async();
+    }
+  }
   if (warp == 1) {
     tmem_alloc2(tmem_base_slot, 512);
     tmem_relinquish2();
   }
   ptx::tc_fence_before();
   __syncthreads();
+  if constexpr (!std::is_same_v<EXT, PPlain>) p_wait_for_previous();
   cluster_sync_all();  // both CTAs' barriers are initialised before any remote arrive or commit can reach them
   ptx::tc_fence_after();
   const uint32_t tmem_base = *tmem_base_slot;
@@ -304,6 +317,13 @@ gemm2_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
       int it = 0;
       bool ok = true;
       uint32_t ag_ready = 0;
+      // A of up to 128 rows: only those are loaded (a load fills rows past the end with zeros, but slowly), the rest of the operand stays zero
+      bool a_none = false;  // this CTA has no rows of A
+      uint32_t stage_bytes = 2 * P_STAGE_BYTES;
+      if constexpr (std::is_same_v<EXT, PCeArgs>) {
+        a_none = M <= P_BLOCK_M && cta == 1;
+        stage_bytes = 2 * P_B_BYTES + (M <= P_BLOCK_M ? 1 : 2) * ext.a_rows * P_BLOCK_K * 2;
+      }
       for (int u = pair; u < sched.total_units && ok; u += num_pairs) {
         const PUnit un = decode_unit(u, sched, k_blocks);
         if (un.kbs <= 0) continue;
@@ -339,12 +359,12 @@ gemm2_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
           if (cta == 0) {
             // the stage is free in both CTAs (the MMAs that read it are complete): tell the peer's producer, then expect both halves
             if (it >= P_STAGES) mbar_arrive_cluster_relaxed(map_to_cta(ptx::smem_u32(&empty_bar[s]), 1));
-            ptx::mbar_expect_tx(&full_bar[s], 2 * P_STAGE_BYTES);
+            ptx::mbar_expect_tx(&full_bar[s], stage_bytes);
           }
           const uint32_t fb = map_to_cta(ptx::smem_u32(&full_bar[s]), 0);  // bytes of both CTAs are counted on the leader's barrier
           if (A_MN) tma2_load_3d(sa, &tmap_a, fb, 0, kb * P_BLOCK_K, m0 / 64);
           else if (a_local) tma2_load_2d(sa, &tmap_al, fb, kb * P_BLOCK_K, m0 - fuse.me * fuse.ag_rows);
-          else      tma2_load_2d(sa, &tmap_a, fb, kb * P_BLOCK_K, m0);
+          else if (!a_none) tma2_load_2d(sa, &tmap_a, fb, kb * P_BLOCK_K, m0);
           if (B_MN) tma2_load_3d(sb, &tmap_b, fb, 0, kb * P_BLOCK_K, n0 / 64);
           else      tma2_load_2d(sb, &tmap_b, fb, kb * P_BLOCK_K, n0);
         }
@@ -690,10 +710,10 @@ EncodeTiledFn p_get_encode() {
   return fn;
 }
 
-bool p_map_kmajor(CUtensorMap* m, const void* ptr, int64_t rows, int64_t k, int64_t ld) {
+bool p_map_kmajor(CUtensorMap* m, const void* ptr, int64_t rows, int64_t k, int64_t ld, int box_rows = P_BLOCK_M) {
   cuuint64_t dims[2] = {(cuuint64_t)k, (cuuint64_t)rows};
   cuuint64_t strides[1] = {(cuuint64_t)ld * 2};
-  cuuint32_t box[2] = {64, 128};
+  cuuint32_t box[2] = {64, (cuuint32_t)box_rows};
   cuuint32_t es[2] = {1, 1};
   return p_get_encode()(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(ptr), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;

@@ -27,6 +27,7 @@ ce_join_kernel(const float2* __restrict__ part, const float* __restrict__ tgt, c
                int rows, float* __restrict__ out_max, float* __restrict__ out_sum, float* __restrict__ out_tgt, float* __restrict__ logz,
                float* __restrict__ loss, float* __restrict__ z, float z_coef) {
   __shared__ float sm[CE_JOIN_PARTS][CE_JOIN_ROWS], ss[CE_JOIN_PARTS][CE_JOIN_ROWS];
+  p_wait_for_previous();
   const int lane = threadIdx.x & 31, grp = threadIdx.x >> 5;
   const int row = blockIdx.x * CE_JOIN_ROWS + lane;
   float m = -INFINITY, s = 0.f;
@@ -82,6 +83,7 @@ __global__ void __launch_bounds__(1024) ce_row_coefficients_kernel(const float* 
 
 // out = bf16(*unit * acc), eight elements a thread.
 __global__ void __launch_bounds__(256) ce_scale_cast_kernel(const float* __restrict__ acc, const float* __restrict__ unit, __nv_bfloat16* __restrict__ out, int64_t n8) {
+  p_wait_for_previous();
   const float u = *unit;
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < n8; i += static_cast<int64_t>(gridDim.x) * 256) {
     Vec8<float> a;
@@ -99,7 +101,7 @@ __global__ void __launch_bounds__(256) ce_scale_cast_kernel(const float* __restr
 // ------------------------------------------------------------------------------------------------ a few tokens
 // Scores of up to 16 tokens: the work is reading the weight once.  A CTA takes 32 whole rows at a time, one contiguous piece of the weight,
 // and neighbouring CTAs neighbouring pieces; the 64-column blocks of the rows are dealt to eight warps, each with a ring of TMA loads of
-// its own, so no warp waits for another but at the end of the 32 rows.  1 x 2048 x 128256: 88 us, 6.0 TB/s (GEMM kernel 150 us); blocks of
+// its own, so no warp waits for another but at the end of the 32 rows.  1 x 2048 x 128256: 85 us, 6.2 TB/s (GEMM kernel 107 us); blocks of
 // 16 rows took 129 us, bound by the turn of a warp's loop (wait, read, four dependent products, next load) rather than by memory.
 //
 // With so few tokens the products are small: mma.sync m16n8k16, 16 weight rows x 8 tokens (bound by the
@@ -161,6 +163,7 @@ ce_few_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant_
     *abort_flag = 0;
     ptx::fence_barrier_init();
   }
+  p_wait_for_previous();
   __syncthreads();
   if (threadIdx.x == 0) {
     ptx::mbar_expect_tx(&bars[0], lay.x_bytes);
@@ -308,6 +311,28 @@ ce_few_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant_
   }
 }
 
+// Launches a kernel that starts with `p_wait_for_previous`: it may be set up while the kernel before it in the stream runs out (saves 1 to 2 us
+// between two kernels of an eager call).  Only behind a kernel that the same entry point has launched: what came before that one is
+// complete by then.
+template <class... P, class... A>
+int ce_launch_next(void (*kern)(P...), int64_t grid, int block, int smem, cudaStream_t stream, A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(grid), 1, 1);
+  cfg.blockDim = dim3(static_cast<unsigned>(block), 1, 1);
+  cfg.dynamicSmemBytes = static_cast<size_t>(smem);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, kern, static_cast<P>(args)...) != cudaSuccess) {
+    cudaGetLastError();
+    return NTB_ERR_LAUNCH;
+  }
+  return ntb_check_launch();
+}
+
 template <class K>
 int ce_configure(K kern, bool (&done)[64], int smem) {
   int dev = 0;
@@ -359,13 +384,15 @@ int ce_launch(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& t
   cfg.blockDim = dim3(p_threads(OUT, EW), 1, 1);
   cfg.dynamicSmemBytes = P_SMEM;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = 2;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // see ce_launch_next
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = OUT == P_OUT_CE_STATS ? 1 : 2;  // the statistics are their entry point's first kernel
   if (cudaLaunchKernelEx(&cfg, kern, ta, tb, td, M, N, K, ce_band(M, K), status, PFuse(), no_maps, sched, tws, ta, ext) != cudaSuccess) {
     cudaGetLastError();
     return NTB_ERR_LAUNCH;
@@ -384,13 +411,18 @@ PSched ce_whole_tiles(int M, int N, int K, bool& fits) {
 }
 
 // Groups of 8 tokens of the few-token kernel, 0: the GEMM kernel.  The tokens' padded copy may take up to 128 KB, the rings the rest.
-// Forward pass, us, this kernel | GEMM kernel: 1 x 2048 x 128256 88 | 150, 16 x 4096 x 128256 177 | 199, 1 x 8192 x 128256 330 | 372; with four
-// groups 32 x 1024 x 128256 took 82 against 80, so more than 16 tokens go to the GEMM kernel.
+// Forward pass, us, this kernel | GEMM kernel: 16 x 256 x 128256 30 | 36, 1 x 2048 x 128256 85 | 107, 16 x 4096 x 128256 172 | 206, 1 x 8192 x
+// 128256 323 | 375; with four groups 32 x 1024 x 128256 took 82 against 65, so more than 16 tokens go to the GEMM kernel.
 int ce_few_groups(int T, int H) {
   if (T > FEW_MAX_TOKENS) return 0;
   const int nt = (T + 7) / 8;
   return static_cast<int64_t>(nt) * 8 * H <= 65536 ? nt : 0;
 }
+
+// Rows of a load of the tokens: no more than there are, in steps of the swizzle's 8 rows.  A load fills rows past the end with zeros, but
+// slowly: forward pass, us, loads of 128 rows | of the tokens: 17 x 1024 x 128256 79 | 64, 17 x 2048 x 128256 128 | 108, 33 x 1024 x 128256 70 |
+// 65, level from 64 tokens on.  What is not loaded has to be zero all the same: leftovers in its place took 4 % (power, not work).
+int ce_a_rows(int T) { return T < P_BLOCK_M ? (T + 7) / 8 * 8 : P_BLOCK_M; }
 
 bool few_map(CUtensorMap* m, const void* ptr, int64_t rows, int64_t k, int64_t ld, int box_rows) {
   cuuint64_t dims[2] = {(cuuint64_t)k, (cuuint64_t)rows};
@@ -414,7 +446,9 @@ int few_launch(const void* x, int64_t ldx, const void* w, int64_t ldw, int T, in
   if (int rc = ce_configure(kern, done, FEW_SMEM)) return rc;
   CUtensorMap tx, tw;
   if (!few_map(&tx, x, T, H, ldx, NT * 8) || !few_map(&tw, w, V, H, ldw, FEW_ROWS)) return NTB_ERR_ARG;
-  kern<<<few_grid(GRAD ? width : V, num_sms), FEW_WARPS * 32, FEW_SMEM, stream>>>(tx, tw, T, V, H / 64, a, static_cast<__nv_bfloat16*>(d), ldd, width, status);
+  __nv_bfloat16* out = static_cast<__nv_bfloat16*>(d);
+  if (GRAD) return ce_launch_next(kern, few_grid(width, num_sms), FEW_WARPS * 32, FEW_SMEM, stream, tx, tw, T, V, H / 64, a, out, ldd, width, status);
+  kern<<<few_grid(V, num_sms), FEW_WARPS * 32, FEW_SMEM, stream>>>(tx, tw, T, V, H / 64, a, out, ldd, width, status);
   return ntb_check_launch();
 }
 template <bool GRAD>
@@ -437,7 +471,8 @@ int ce_stats(const void* x, int64_t ldx, const void* w, int64_t ldw, const int64
   bool fits;
   const PSched sched = ce_whole_tiles(T, V, H, fits);
   CUtensorMap ta, tb;
-  if (!fits || !p_map_kmajor(&ta, x, T, H, ldx) || !p_map_kmajor(&tb, w, V, H, ldw)) return NTB_ERR_ARG;
+  a.a_rows = ce_a_rows(T);
+  if (!fits || !p_map_kmajor(&ta, x, T, H, ldx, a.a_rows) || !p_map_kmajor(&tb, w, V, H, ldw)) return NTB_ERR_ARG;
   return ce_launch<false, false, P_OUT_CE_STATS>(ta, tb, ta, T, V, H, sched, ta, a, status, num_sms, stream);
 }
 
@@ -455,7 +490,8 @@ int ce_dlogits(const void* x, int64_t ldx, const void* w, int64_t ldw, const int
   bool fits;
   const PSched sched = ce_whole_tiles(T, V, H, fits);
   CUtensorMap ta, tb, td;
-  if (!fits || !p_map_kmajor(&ta, x, T, H, ldx) || !p_map_kmajor(&tb, w, V, H, ldw) || !p_map_out(&td, d, T, width, ldd, false)) return NTB_ERR_ARG;
+  a.a_rows = ce_a_rows(T);
+  if (!fits || !p_map_kmajor(&ta, x, T, H, ldx, a.a_rows) || !p_map_kmajor(&tb, w, V, H, ldw) || !p_map_out(&td, d, T, width, ldd, false)) return NTB_ERR_ARG;
   return ce_launch<false, false, P_OUT_CE_GRAD>(ta, tb, td, T, V, H, sched, ta, a, status, num_sms, stream);
 }
 
@@ -464,6 +500,7 @@ int ce_dlogits(const void* x, int64_t ldx, const void* w, int64_t ldw, const int
 // the sum takes its parallelism from the rows.
 __global__ void __launch_bounds__(256) ce_split_sum_kernel(const float* __restrict__ ws, void* __restrict__ out, int64_t ldo, int M, int N, int split, int chunks, int tiles_m,
                                                             int tiles_n, int band, int bf16_out, int accumulate, const float* __restrict__ unit) {
+  p_wait_for_previous();
   const int tile = blockIdx.x >> 5;
   const PTile tc = pair_tile(tile, tiles_m, tiles_n, band);
   const int r = (blockIdx.x & 31) * 8 + (threadIdx.x >> 5), c8 = (threadIdx.x & 31) * 8;
@@ -528,8 +565,8 @@ int ce_dx(const void* d, int64_t ldd, const void* w, int64_t ldw, void* dx, int6
   else rc = ce_launch<false, true, P_OUT_F32_ACCUM>(ta, tb, td, T, H, V, sched, tws, a, status, num_sms, stream);
   if (rc != NTB_OK || split == 1) return rc;
   const int chunks = (kb + sched.kb_per - 1) / sched.kb_per;  // chunks past the end of K wrote nothing
-  ce_split_sum_kernel<<<tiles * 32, 256, 0, stream>>>(ws, dx, lddx, T, H, split, chunks, (T + 255) / 256, (H + 255) / 256, ce_band(T, V), mode == 0, mode == 2, unit);
-  return ntb_check_launch();
+  return ce_launch_next(ce_split_sum_kernel, tiles * 32, 256, 0, stream, ws, dx, lddx, T, H, split, chunks, (T + 255) / 256, (H + 255) / 256, ce_band(T, V), mode == 0, mode == 2,
+                        unit);
 }
 
 // Rows of the weight gradient: dw [V, H] = unit * d^T x (accumulate 0: bf16 store; 1: added to fp32 dw).
@@ -561,10 +598,9 @@ NTB_EXPORT int ntb_linear_ce_forward(const void* x, int64_t ldx, const void* w, 
   float* tgt = part + static_cast<int64_t>(tiles) * 2 * T;
   const int rc = ce_stats(x, ldx, w, ldw, target, vocab_start, T, V, H, part, tgt, status, num_sms, stream);
   if (rc != NTB_OK) return rc;
-  ce_join_kernel<<<(T + CE_JOIN_ROWS - 1) / CE_JOIN_ROWS, CE_JOIN_ROWS * CE_JOIN_PARTS, 0, stream>>>(
-      reinterpret_cast<const float2*>(part), tgt, target, vocab_start, V, tiles, T, finish ? nullptr : out0, finish ? nullptr : out1, finish ? nullptr : out2,
-      finish ? out0 : nullptr, finish ? out1 : nullptr, finish && z_coef > 0.f ? out2 : nullptr, z_coef);
-  return ntb_check_launch();
+  return ce_launch_next(ce_join_kernel, (T + CE_JOIN_ROWS - 1) / CE_JOIN_ROWS, CE_JOIN_ROWS * CE_JOIN_PARTS, 0, stream, reinterpret_cast<const float2*>(part), tgt, target,
+                        vocab_start, V, tiles, T, finish ? nullptr : out0, finish ? nullptr : out1, finish ? nullptr : out2, finish ? out0 : nullptr, finish ? out1 : nullptr,
+                        finish && z_coef > 0.f ? out2 : nullptr, z_coef);
 }
 
 // How the dx product [T, H] over V is cut along V: with fewer tiles than CTA pairs (few tokens) every tile becomes `split` chunks
@@ -618,7 +654,7 @@ NTB_EXPORT int ntb_linear_ce_backward(const void* x, int64_t ldx, const void* w,
   if (dx != nullptr && width < V) {
     const int64_t n8 = static_cast<int64_t>(T) * H / 8;
     const int64_t blocks = (n8 + 255) / 256;
-    ce_scale_cast_kernel<<<static_cast<unsigned>(blocks < 148 * 8 ? blocks : 148 * 8), 256, 0, stream>>>(acc, unit, static_cast<__nv_bfloat16*>(dx), n8);
+    return ce_launch_next(ce_scale_cast_kernel, blocks < 148 * 8 ? blocks : 148 * 8, 256, 0, stream, acc, unit, static_cast<__nv_bfloat16*>(dx), n8);
   }
   return ntb_check_launch();
 }

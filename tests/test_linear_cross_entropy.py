@@ -191,6 +191,8 @@ def check(x, w, y, g, z=0.0, main_grad=None):
 SHAPES = [(1, 64, 1), (1, 64, 257), (3, 128, 255), (2, 192, 64), (257, 64, 1000), (128, 448, 4096), (130, 4096, 513), (515, 576, 9001), (64, 1024, 20011), (2049, 128, 777), (300, 1088, 1000), (257, 4096, 700), (40, 2112, 3000)]
 # up to 16 tokens that fit beside the rings take their own kernel: its token groups, odd block counts, last rows, and the sizes just past it
 SHAPES += [(1, 2048, 5003), (8, 8192, 300), (9, 4096, 1000), (16, 4160, 129), (17, 64, 16), (31, 576, 2400), (32, 2048, 4111), (33, 64, 100), (7, 64, 40000), (1, 8256, 33)]
+# GEMM kernel with operands of fewer rows than a load takes otherwise
+SHAPES += [(24, 4096, 600), (113, 320, 1500), (121, 1152, 260), (127, 64, 70000), (129, 1088, 300)]
 
 
 @gpu
