@@ -12,7 +12,7 @@
 // cta_group::2 form of cp.async.bulk.tensor, whose completion bytes are counted on the LEADER's stage barrier, so the leader's MMA
 // thread waits on one barrier for both halves); warp 1: the MMA issuer in the leader, idle in the peer; warps 2..5 epilogue
 // (tcgen05.ld -> swizzled staging -> TMA store / reduce-add of the CTA's own rows).  Epilogues that compute take EW = 8 warps, four to
-// each half of the columns: 2..9, or 4..11 with warps 2 and 3 idle where warp groups exchange registers (P_OUT_CE_STATS).
+// each half of the columns: 2..9, or 4..11 with warps 2 and 3 idle where warp groups exchange registers (statistics).
 // Cross-CTA signals besides the loads are plain remote mbarrier arrives: the leader's producer forwards every "stage free" to the
 // peer's producer, one leader epilogue warp forwards "accumulator ready" to the peer's epilogue, and the peer's epilogue warps hand
 // accumulators back to the leader's MMA thread.  All waits are bounded; the two CTAs meet in a cluster barrier before TMEM is freed.
@@ -37,7 +37,8 @@ constexpr int P_EPI_BUF = 32 * 128;
 constexpr int P_THREADS = 32 * (2 + P_EPI_WARPS);
 constexpr int P_SMEM = P_MAX_STAGES * P_STAGE_BYTES + P_EPI_WARPS * 2 * P_EPI_BUF + 1024 + 512;
 
-enum POut { P_OUT_BF16 = 0, P_OUT_F32 = 1, P_OUT_F32_ACCUM = 2, P_OUT_PEER_BF16 = 3, P_OUT_CE_STATS = 4, P_OUT_CE_GRAD = 5 };
+enum POut { P_OUT_BF16 = 0, P_OUT_F32 = 1, P_OUT_F32_ACCUM = 2, P_OUT_PEER_BF16 = 3, P_OUT_CE_STATS = 4, P_OUT_CE_GRAD = 5, P_OUT_CE_STATS_T = 6 };
+constexpr bool p_ce_stats(int out) { return out == P_OUT_CE_STATS || out == P_OUT_CE_STATS_T; }
 
 // What an epilogue needs beside the accumulator.  PPlain: nothing.
 struct PPlain {};
@@ -50,14 +51,22 @@ struct PAlpha {
 struct PCeArgs {
   const int64_t* target = nullptr;  // [M] class of every row, in the numbering in which column 0 of this product is `col0`
   int64_t col0 = 0;
-  int a_rows = P_BLOCK_M;           // rows per load of A: P_BLOCK_M, or all there are in steps of 8
   // P_OUT_CE_STATS: nothing but these leaves the kernel
   float2* part = nullptr;           // [tiles_n * EW / 4][M] (largest score, sum exp(score - largest)) of every 1024 / EW columns
   float* tgt = nullptr;             // [M] the target's score, written where the target is one of this product's columns
+  // P_OUT_CE_STATS_T: the product the other way around, A = rows of the head weight, B = hidden states, so that a tile's width follows the
+  // number of tokens (`tile_n`, a multiple of 32 up to 256; `part` is then [2 pairs of a token tile][N], `target` and `tgt` are [N])
+  int tile_n = P_BLOCK_N;
   // P_OUT_CE_GRAD: D = coef * exp(score - logz) - g * [column is the target], zero in the padding columns of D
   const float* logz = nullptr;
   const float* coef = nullptr;
   const float* g = nullptr;
+  int a_rows = P_BLOCK_M;           // rows per load of A: P_BLOCK_M, or all there are in steps of 8
+};
+
+// P_OUT_CE_STATS_T: BLOCKS = tile_n / 64, rounded up.
+template <int BLOCKS_> struct PCeTurned : PCeArgs {
+  static constexpr int BLOCKS = BLOCKS_;
 };
 
 // The tensor cores cut what does not fit when they add to an accumulator: a sum over K comes out small by about 2^-26 of its value per 16
@@ -236,13 +245,13 @@ __device__ __forceinline__ void p_ce_gradient(uint32_t (&r)[32], int valid, int 
   }
 }
 
-// P_OUT_CE_STATS keeps 128 scores of a row in every epilogue thread.  Its warps come in groups of four that exchange registers: the
+// The statistics keep 128 scores of a row in every epilogue thread.  Its warps come in groups of four that exchange registers: the
 // first group (producer, MMA issuer, two idle warps) hands most of its own to the two epilogue groups.  The shares add up to what the
 // block is launched with (168 x 384); the host checks that before the launch.  (Without the exchange the scores spill, 168 registers at
 // eight or 96 at sixteen epilogue warps, and the pass takes 1.3 times as long.)
 constexpr int P_SPLIT_REGS = 168, P_SPLIT_REGS_LOAD = 72, P_SPLIT_REGS_EPI = 216;
 static_assert(4 * P_SPLIT_REGS_LOAD + 8 * P_SPLIT_REGS_EPI == 12 * P_SPLIT_REGS, "register shares of the warp groups");
-constexpr int p_first_epilogue_warp(int out) { return out == P_OUT_CE_STATS ? 4 : 2; }
+constexpr int p_first_epilogue_warp(int out) { return p_ce_stats(out) ? 4 : 2; }
 constexpr int p_threads(int out, int ew) { return 32 * (p_first_epilogue_warp(out) + ew); }
 
 // EW: epilogue warps per CTA, 4 (each takes 32 rows), or in the cross entropy modes 8 (each takes 32 rows and half of the columns; where
@@ -255,13 +264,17 @@ gemm2_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
                      const __grid_constant__ EXT ext) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  constexpr int EPI_BYTES = OUT == P_OUT_CE_STATS ? 0 : EW * 2 * P_EPI_BUF;
-  static_assert(P_STAGES * P_STAGE_BYTES + EPI_BYTES + 1024 + 512 <= P_SMEM && P_STAGES <= P_MAX_STAGES && (EW == 4 || (EW == 8 && (OUT == P_OUT_CE_STATS || OUT == P_OUT_CE_GRAD))), "shared memory of a launch");
-  uint8_t* epi_smem = smem + P_STAGES * P_STAGE_BYTES;
+  constexpr bool TURNED = OUT == P_OUT_CE_STATS_T;  // more stages where they are smaller
+  constexpr int STAGE = TURNED ? P_MAX_STAGES * P_STAGE_BYTES / P_STAGES : P_STAGE_BYTES;
+  constexpr int EPI_BYTES = OUT == P_OUT_CE_STATS ? 0 : TURNED ? EW * P_EPI_BUF : EW * 2 * P_EPI_BUF;
+  static_assert(P_STAGES * STAGE + EPI_BYTES + 1024 + 512 <= P_SMEM && P_STAGES <= 2 * P_MAX_STAGES && STAGE % 1024 == 0 &&
+                    (EW == 4 || (EW == 8 && (p_ce_stats(OUT) || OUT == P_OUT_CE_GRAD))),
+                "shared memory of a launch");
+  uint8_t* epi_smem = smem + P_STAGES * STAGE;
   uint64_t* bars = reinterpret_cast<uint64_t*>(epi_smem + EPI_BYTES);
   uint64_t* full_bar = bars;                       // [STAGES]  (leader) both CTAs' loads of the stage have landed
   uint64_t* empty_bar = bars + 2 * P_MAX_STAGES;       // [STAGES]  the MMAs that read this stage are done
-  uint64_t* tmem_full = bars + 3 * P_MAX_STAGES;       // [2]
+  uint64_t* tmem_full = bars + 4 * P_MAX_STAGES;       // [2]
   uint64_t* tmem_empty = tmem_full + 2;            // [2]  (leader) both CTAs' epilogues have drained the accumulator
   uint32_t* tmem_base_slot = reinterpret_cast<uint32_t*>(tmem_empty + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_base_slot + 1);
@@ -273,7 +286,9 @@ gemm2_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
   const int pair = blockIdx.x >> 1;
   const int num_pairs = gridDim.x >> 1;
   const int tiles_m = (M + 2 * P_BLOCK_M - 1) / (2 * P_BLOCK_M);
-  const int tiles_n = (N + P_BLOCK_N - 1) / P_BLOCK_N;
+  int block_n = P_BLOCK_N;
+  if constexpr (TURNED) block_n = ext.tile_n;
+  const int tiles_n = (N + block_n - 1) / block_n;
   const int k_blocks = (K + P_BLOCK_K - 1) / P_BLOCK_K;
 
   if (threadIdx.x == 0) {
@@ -291,7 +306,7 @@ gemm2_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
     ptx::prefetch_tmap(&tmap_b);
     ptx::prefetch_tmap(&tmap_d);
   }
-  if constexpr (std::is_same_v<EXT, PCeArgs>) {
+  if constexpr (OUT == P_OUT_CE_GRAD) {
     if (M <= P_BLOCK_M) {  // rows of A that no load fills
       for (int i = threadIdx.x; i < P_STAGES * (P_A_BYTES / 16); i += blockDim.x)
         *reinterpret_cast<uint4*>(smem + (i / (P_A_BYTES / 16)) * P_STAGE_BYTES + (i % (P_A_BYTES / 16)) * 16) = make_uint4(0, 0, 0, 0);
@@ -310,7 +325,7 @@ gemm2_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
   const uint32_t tmem_base = *tmem_base_slot;
 
   if (warp < EPI0) {
-  if constexpr (OUT == P_OUT_CE_STATS) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(P_SPLIT_REGS_LOAD));
+  if constexpr (p_ce_stats(OUT)) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(P_SPLIT_REGS_LOAD));
   if (warp == 0) {
     // ------------------------------------------------------------------ TMA producer (both CTAs)
     if (ptx::elect_one()) {
@@ -320,17 +335,19 @@ gemm2_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
       // A of up to 128 rows: only those are loaded (a load fills rows past the end with zeros, but slowly), the rest of the operand stays zero
       bool a_none = false;  // this CTA has no rows of A
       uint32_t stage_bytes = 2 * P_STAGE_BYTES;
-      if constexpr (std::is_same_v<EXT, PCeArgs>) {
+      if constexpr (TURNED) {
+        stage_bytes = 2 * P_A_BYTES + block_n * P_BLOCK_K * 2;
+      } else if constexpr (OUT == P_OUT_CE_GRAD) {
         a_none = M <= P_BLOCK_M && cta == 1;
         stage_bytes = 2 * P_B_BYTES + (M <= P_BLOCK_M ? 1 : 2) * ext.a_rows * P_BLOCK_K * 2;
       }
       for (int u = pair; u < sched.total_units && ok; u += num_pairs) {
         const PUnit un = decode_unit(u, sched, k_blocks);
         if (un.kbs <= 0) continue;
-        PTile tc = pair_tile(un.tile, tiles_m, tiles_n, band);
+        PTile tc = TURNED ? PTile{un.tile / tiles_n, un.tile % tiles_n} : pair_tile(un.tile, tiles_m, tiles_n, band);
         tc.m_blk = (tc.m_blk + fuse.m_rot) % tiles_m;
         const int m0 = (tc.m_blk * 2 + static_cast<int>(cta)) * P_BLOCK_M;           // this CTA's rows of A
-        const int n0 = tc.n_blk * P_BLOCK_N + static_cast<int>(cta) * P_HALF_N;      // this CTA's half of B
+        const int n0 = tc.n_blk * block_n + static_cast<int>(cta) * (block_n / 2);   // this CTA's half of B
         bool a_local = false;
         if (fuse.ag_flags != nullptr && m0 < M) {
           const int src = min(fuse.world - 1, m0 / fuse.ag_rows);  // ag_rows is a multiple of 128: one source per CTA row block
@@ -354,7 +371,7 @@ gemm2_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
           const int s = it % P_STAGES;
           const uint32_t ph = (it / P_STAGES) & 1;
           if (!ptx::mbar_wait(&empty_bar[s], ph ^ 1, abort_flag, 200)) { ok = false; break; }
-          uint8_t* sa = smem + s * P_STAGE_BYTES;
+          uint8_t* sa = smem + s * STAGE;
           uint8_t* sb = sa + P_A_BYTES;
           if (cta == 0) {
             // the stage is free in both CTAs (the MMAs that read it are complete): tell the peer's producer, then expect both halves
@@ -388,15 +405,15 @@ gemm2_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
     if (ptx::elect_one()) {
       if (cta == 0) {
         // ---------------------------------------------------------------- MMA issuer (leader)
-        constexpr uint32_t idesc = ptx::make_idesc_bf16(2 * P_BLOCK_M, P_BLOCK_N, A_MN, B_MN);
+        const uint32_t idesc = ptx::make_idesc_bf16(2 * P_BLOCK_M, block_n, A_MN, B_MN);
         int it = 0, tile_it = 0;
         bool ok = true;
         for (int u = pair; u < sched.total_units && ok; u += num_pairs) {
           const PUnit un = decode_unit(u, sched, k_blocks);
           if (un.kbs <= 0) continue;
           int kb = 0;
-          do {  // one accumulator per tile; P_OUT_CE_STATS: one per P_CE_SEGMENT k-blocks of a tile
-            const int kb0 = kb, kb1 = OUT == P_OUT_CE_STATS ? min(kb + P_CE_SEGMENT, un.kbs) : un.kbs;
+          do {  // one accumulator per tile; statistics: one per P_CE_SEGMENT k-blocks of a tile
+            const int kb0 = kb, kb1 = p_ce_stats(OUT) ? min(kb + P_CE_SEGMENT, un.kbs) : un.kbs;
             const int acc = tile_it & 1;
             const uint32_t acc_ph = (tile_it >> 1) & 1;
             tile_it++;
@@ -408,7 +425,7 @@ gemm2_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
               const uint32_t ph = (it / P_STAGES) & 1;
               if (!ptx::mbar_wait(&full_bar[s], ph, abort_flag)) { ok = false; break; }
               ptx::tc_fence_after();
-              const uint32_t sa = ptx::smem_u32(smem + s * P_STAGE_BYTES);
+              const uint32_t sa = ptx::smem_u32(smem + s * STAGE);
               const uint32_t sb = sa + P_A_BYTES;
   #pragma unroll
               for (int k = 0; k < P_BLOCK_K / P_UMMA_K; k++) {
@@ -419,15 +436,15 @@ gemm2_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
               umma2_commit(ptx::smem_u32(&empty_bar[s]));  // the stage is free once these MMAs (in both SMs) have read it
             }
             if (ok) umma2_commit(ptx::smem_u32(&tmem_full[acc]));
-          } while (OUT == P_OUT_CE_STATS && ok && kb < un.kbs);
+          } while (p_ce_stats(OUT) && ok && kb < un.kbs);
         }
       }
     }
   }
   } else {
-    if constexpr (OUT == P_OUT_CE_STATS) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(P_SPLIT_REGS_EPI));
+    if constexpr (p_ce_stats(OUT)) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(P_SPLIT_REGS_EPI));
     // ------------------------------------------------------------------ epilogue warps (both CTAs, own 128 rows)
-    constexpr uint32_t POLL_NS = OUT == P_OUT_CE_STATS ? 100 : 1000;  // pieces of a tile follow one another in 4 us
+    constexpr uint32_t POLL_NS = p_ce_stats(OUT) ? 100 : 1000;  // pieces of a tile follow one another in 4 us
     const int q = warp & 3;
     const int half = EW == 8 ? (warp - EPI0) >> 2 : 0;  // of the columns
     uint8_t* my_epi = epi_smem + (warp - EPI0) * 2 * P_EPI_BUF;
@@ -436,6 +453,100 @@ gemm2_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
     if constexpr (std::is_same_v<EXT, PAlpha>) alpha = ext.alpha ? *ext.alpha : 1.f;
     int tile_it = 0, buf = 0;
     bool ok = true;
+    if constexpr (TURNED) {
+      // A warp has 32 vocabulary entries (lanes) of up to 128 tokens (columns), always the same tokens: the grid is a multiple of the token
+      // tiles.  Blocks of 32 x 32 scores are turned around in shared memory, so that a lane folds 32 scores of its own token into running
+      // statistics that stay in registers until the CTA's last tile.
+      constexpr int NB = EXT::BLOCKS;  // blocks of 32 columns; the second half of the warps may have one without tokens at its end
+      const int n_blk = pair % tiles_n, c0 = half * NB * 32;
+      float* turn = reinterpret_cast<float*>(epi_smem + (warp - EPI0) * P_EPI_BUF);
+      float m[NB], s[NB];
+      int tl[NB];  // the token's target among this product's rows, or far from any row
+#pragma unroll
+      for (int b = 0; b < NB; b++) {
+        m[b] = -INFINITY;
+        s[b] = 0.f;
+        tl[b] = -(1 << 30);
+        const int col = c0 + b * 32 + lane, token = n_blk * block_n + col;
+        if (col < block_n && token < N) {
+          const int64_t rel = ext.target[token] - ext.col0;
+          if (rel >= 0 && rel < M) tl[b] = static_cast<int>(rel);
+        }
+      }
+      auto hand_back = [&](int a) {
+        ptx::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          if (cta == 0) ptx::mbar_arrive(&tmem_empty[a]);
+          else mbar_arrive_cluster(map_to_cta(ptx::smem_u32(&tmem_empty[a]), 0));
+        }
+      };
+      for (int u = pair; u < sched.total_units && ok; u += num_pairs) {
+        const int row0 = (u / tiles_n * 2 + static_cast<int>(cta)) * P_BLOCK_M + q * 32;
+        const int valid = M - row0;  // rows that exist: the others are zeros of the load
+        auto fold = [&](int b, const uint32_t (&r)[32]) {
+#pragma unroll
+          for (int j = 0; j < 8; j++)
+            *reinterpret_cast<uint4*>(turn + lane * 32 + ((j ^ (lane & 7)) << 2)) = make_uint4(r[j * 4], r[j * 4 + 1], r[j * 4 + 2], r[j * 4 + 3]);
+          __syncwarp();
+          auto at = [&](int i) { return turn + i * 32 + (((lane >> 2) ^ (i & 7)) << 2) + (lane & 3); };
+          const int i = tl[b] - row0;
+          if (i >= 0 && i < 32) ext.tgt[n_blk * block_n + c0 + b * 32 + lane] = *at(i);
+#pragma unroll 1
+          for (int h = 0; h < 32; h += 16) {
+            uint32_t own[16];
+#pragma unroll
+            for (int i = 0; i < 16; i++) own[i] = __float_as_uint(*at(h + i));
+            p_ce_accumulate(own, valid - h, m[b], s[b]);
+          }
+          __syncwarp();
+        };
+        uint32_t sums[NB][32];
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+          for (int j = 0; j < 32; j++) sums[b][j] = 0u;
+        for (int kb = 0; kb < k_blocks; kb += P_CE_SEGMENT) {
+          const int a = tile_it & 1;
+          if (!ptx::mbar_wait(&tmem_full[a], (tile_it >> 1) & 1, abort_flag, POLL_NS)) { ok = false; break; }
+          tile_it++;
+          if (cta == 0 && warp == EPI0 && lane == 0) mbar_arrive_cluster(map_to_cta(ptx::smem_u32(&tmem_full[a]), 1));  // forward to the peer's epilogue
+          ptx::tc_fence_after();
+          const uint32_t ta = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + a * P_BLOCK_N + c0;
+#pragma unroll
+          for (int b = 0; b < NB; b++) {
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+              uint32_t r0[8];
+              ptx::tmem_ld_32x8(ta + b * 32 + c * 8, r0);
+              ptx::tmem_ld_wait();
+#pragma unroll
+              for (int j = 0; j < 8; j++) sums[b][c * 8 + j] = __float_as_uint(__uint_as_float(sums[b][c * 8 + j]) + __uint_as_float(r0[j]));
+            }
+          }
+          hand_back(a);
+        }
+        if (!ok) break;
+#pragma unroll
+        for (int b = 0; b < NB; b++) fold(b, sums[b]);
+      }
+      // the four row groups of the CTA
+      float2* all = reinterpret_cast<float2*>(epi_smem);  // [4][256]
+      asm volatile("bar.sync 1, %0;" ::"n"(32 * EW) : "memory");
+#pragma unroll
+      for (int b = 0; b < NB; b++) all[q * 256 + c0 + b * 32 + lane] = make_float2(m[b], s[b]);
+      asm volatile("bar.sync 1, %0;" ::"n"(32 * EW) : "memory");
+      const int e = threadIdx.x - EPI0 * 32, token = n_blk * block_n + e;
+      if (e < block_n && token < N) {
+        float gm = -INFINITY, gs = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; i++) gm = fmaxf(gm, all[i * 256 + e].x);
+        const float base = gm == -INFINITY ? 0.f : gm * P_LOG2E;
+#pragma unroll
+        for (int i = 0; i < 4; i++) gs += all[i * 256 + e].y * p_ex2(fmaf(all[i * 256 + e].x, P_LOG2E, -base));
+        ext.part[static_cast<int64_t>(pair / tiles_n * 2 + static_cast<int>(cta)) * N + token] = make_float2(gm, gs);
+      }
+    } else
     for (int u = pair; u < sched.total_units && ok; u += num_pairs) {
       const PUnit un = decode_unit(u, sched, k_blocks);
       if (un.kbs <= 0) continue;
@@ -610,7 +721,7 @@ gemm2_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
         buf ^= 1;
       }
       }
-      if constexpr (OUT != P_OUT_CE_STATS) {
+      if constexpr (!p_ce_stats(OUT)) {
         // accumulator fully read: hand it back to the leader's MMA thread (a remote arrive from the peer CTA)
         ptx::tc_fence_before();
         __syncwarp();

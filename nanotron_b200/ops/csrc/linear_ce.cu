@@ -4,7 +4,8 @@
 //   d[t,v] = coef[t] exp(l[t,v] - logZ[t]) - g[t] [v == y_t]             dx = d w        dw = d^T x
 //
 // Forward: one GEMM over the whole vocabulary on CTA pairs (gemm2_core.cuh) whose epilogue keeps, per token and 256-column tile, only
-// (largest score, sum of exponentials); a small kernel joins the half tiles of a token.  Scores never leave the tensor memory, and they
+// (largest score, sum of exponentials); a small kernel joins the half tiles of a token.  With few tokens the operands change places (up to
+// 1024, see ce_turned_tile) or the weight is only streamed (up to 8, ce_few_kernel).  Scores never leave the tensor memory, and they
 // are used in fp32 (logits written in bf16 are off by up to 2^-8 of their value, several percent of a probability).  They are accumulated
 // 1024 products at a time and the pieces added in registers, because the tensor cores cut when they add to an accumulator: a score comes
 // out small by 1e-6 of its value at any H (in one accumulator by 9e-10 H), the loss of scores with a standard deviation of 1.5 by 3e-7 (in
@@ -99,9 +100,9 @@ __global__ void __launch_bounds__(256) ce_scale_cast_kernel(const float* __restr
 }
 
 // ------------------------------------------------------------------------------------------------ a few tokens
-// Scores of up to 16 tokens: the work is reading the weight once.  A CTA takes 32 whole rows at a time, one contiguous piece of the weight,
+// Scores of up to 8 tokens: the work is reading the weight once.  A CTA takes 32 whole rows at a time, one contiguous piece of the weight,
 // and neighbouring CTAs neighbouring pieces; the 64-column blocks of the rows are dealt to eight warps, each with a ring of TMA loads of
-// its own, so no warp waits for another but at the end of the 32 rows.  1 x 2048 x 128256: 85 us, 6.2 TB/s (GEMM kernel 107 us); blocks of
+// its own, so no warp waits for another but at the end of the 32 rows.  1 x 2048 x 128256: 85 us, 6.2 TB/s; blocks of
 // 16 rows took 129 us, bound by the turn of a warp's loop (wait, read, four dependent products, next load) rather than by memory.
 //
 // With so few tokens the products are small: mma.sync m16n8k16, 16 weight rows x 8 tokens (bound by the
@@ -112,18 +113,18 @@ __global__ void __launch_bounds__(256) ce_scale_cast_kernel(const float* __restr
 constexpr int FEW_WARPS = 8;
 constexpr int FEW_ROWS = 32;
 constexpr int FEW_SLOT = FEW_ROWS * 128;  // bytes of one 32 x 64 block
-constexpr int FEW_MAX_TOKENS = 16;
+constexpr int FEW_TOKENS = 8;
 constexpr int FEW_MAX_STAGES = 8;
 constexpr int FEW_SMEM = 227 * 1024;
 
 struct FewLayout {  // of the dynamic shared memory, from a 1024-byte boundary on
   int x_bytes, red_bytes, stages;
 };
-// NT: groups of 8 tokens.  Partial sums of the warps go through two buffers (one CTA barrier per 32 rows).
-__host__ __device__ inline FewLayout few_layout(int nt, int k_blocks) {
+// Partial sums of the warps go through two buffers (one CTA barrier per 32 rows).
+__host__ __device__ inline FewLayout few_layout(int k_blocks) {
   FewLayout l;
-  l.x_bytes = k_blocks * nt * 1024;
-  l.red_bytes = 2 * FEW_WARPS * FEW_ROWS * 8 * nt * 4;
+  l.x_bytes = k_blocks * FEW_TOKENS * 128;
+  l.red_bytes = 2 * FEW_WARPS * FEW_ROWS * FEW_TOKENS * 4;
   const int left = FEW_SMEM - 2048 - l.x_bytes - l.red_bytes;
   l.stages = left / (FEW_WARPS * FEW_SLOT);
   if (l.stages > FEW_MAX_STAGES) l.stages = FEW_MAX_STAGES;
@@ -142,13 +143,13 @@ __device__ __forceinline__ uint4 few_word(const uint8_t* block, int row, int wor
 
 // GRAD false: part[blockIdx.x][T] = (largest, sum of exponentials) of the rows this CTA saw, and the targets' scores.  GRAD true:
 // d [T, V] at pitch ldd, columns up to `width` written.
-template <int NT, bool GRAD>
+template <bool GRAD>
 __global__ void __launch_bounds__(FEW_WARPS * 32, 1)
 ce_few_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w, int T, int V, int k_blocks, PCeArgs args, __nv_bfloat16* __restrict__ d,
               int64_t ldd, int width, int* __restrict__ status) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  const FewLayout lay = few_layout(NT, k_blocks);
+  const FewLayout lay = few_layout(k_blocks);
   uint8_t* xs = smem;
   uint8_t* ring = xs + lay.x_bytes;
   float* red = reinterpret_cast<float*>(ring + lay.stages * FEW_WARPS * FEW_SLOT);
@@ -167,7 +168,7 @@ ce_few_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant_
   __syncthreads();
   if (threadIdx.x == 0) {
     ptx::mbar_expect_tx(&bars[0], lay.x_bytes);
-    for (int kb = 0; kb < k_blocks; kb++) ptx::tma_load_2d(xs + kb * NT * 1024, &tmap_x, &bars[0], kb * 64, 0);
+    for (int kb = 0; kb < k_blocks; kb++) ptx::tma_load_2d(xs + kb * FEW_TOKENS * 128, &tmap_x, &bars[0], kb * 64, 0);
   }
   // this warp's blocks, in order: for each of the CTA's groups, blocks warp, warp + 8, ...
   const int per_group = k_blocks > warp ? (k_blocks - warp + FEW_WARPS - 1) / FEW_WARPS : 0;
@@ -188,35 +189,27 @@ ce_few_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant_
     while (next < total && next < lay.stages) issue();
   bool ok = __all_sync(0xffffffffu, ptx::mbar_wait(&bars[0], 0, abort_flag));
 
-  // thread -> (row, token) of the 32 x 8 NT scores, for the epilogue
-  constexpr int OWN = (FEW_ROWS * 8 * NT + FEW_WARPS * 32 - 1) / (FEW_WARPS * 32);
-  float run_m[OWN], run_s[OWN], e_lz[OWN], e_coef[OWN], e_g[OWN];
-  int e_t[OWN];
-#pragma unroll
-  for (int o = 0; o < OWN; o++) {
-    run_m[o] = -INFINITY;
-    run_s[o] = e_lz[o] = e_coef[o] = e_g[o] = 0.f;
-    e_t[o] = -1;
-    const int token = (threadIdx.x + o * FEW_WARPS * 32) / FEW_ROWS;
-    if (token < T) {
-      const int64_t rel = args.target[token] - args.col0;
-      if (rel >= 0 && rel < V) e_t[o] = static_cast<int>(rel);
-      if (GRAD) {
-        e_lz[o] = args.logz[token] * P_LOG2E;
-        e_coef[o] = args.coef[token];
-        e_g[o] = args.g[token];
-      }
+  // the epilogue gives every thread one of the 32 x 8 scores: a warp has the 32 rows of a token
+  static_assert(FEW_WARPS == FEW_TOKENS && FEW_ROWS == 32, "threads of the epilogue");
+  const int token = warp;
+  float run_m = -INFINITY, run_s = 0.f, e_lz = 0.f, e_coef = 0.f, e_g = 0.f;
+  int e_t = -1;
+  if (token < T) {
+    const int64_t rel = args.target[token] - args.col0;
+    if (rel >= 0 && rel < V) e_t = static_cast<int>(rel);
+    if (GRAD) {
+      e_lz = args.logz[token] * P_LOG2E;
+      e_coef = args.coef[token];
+      e_g = args.g[token];
     }
   }
 
   int slot = 0, buf = 0;
   uint32_t phase = 0;
   for (int group = blockIdx.x; group < groups; group += gridDim.x) {
-    float acc[2][NT][4];
+    float acc[2][4];
 #pragma unroll
-    for (int n = 0; n < NT; n++)
-#pragma unroll
-      for (int j = 0; j < 4; j++) acc[0][n][j] = acc[1][n][j] = 0.f;
+    for (int j = 0; j < 4; j++) acc[0][j] = acc[1][j] = 0.f;
     for (int kb = warp; kb < k_blocks && ok; kb += FEW_WARPS) {
       if (!__all_sync(0xffffffffu, ptx::mbar_wait(&my_bars[slot], phase, abort_flag))) { ok = false; break; }
       const uint8_t* blk = my_ring + slot * FEW_SLOT;
@@ -228,55 +221,47 @@ ce_few_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant_
         w[m][2] = few_word(blk, m * 16 + g + 8, 2 * t);
         w[m][3] = few_word(blk, m * 16 + g + 8, 2 * t + 1);
       }
+      const uint8_t* xb = xs + kb * FEW_TOKENS * 128;
+      const uint4 b0 = few_word(xb, g, 2 * t), b1 = few_word(xb, g, 2 * t + 1);
 #pragma unroll
-      for (int n = 0; n < NT; n++) {
-        const uint8_t* xb = xs + (kb * NT + n) * 1024;
-        const uint4 b0 = few_word(xb, g, 2 * t), b1 = few_word(xb, g, 2 * t + 1);
+      for (int m = 0; m < 2; m++) few_mma(acc[m], w[m][0].x, w[m][2].x, w[m][0].y, w[m][2].y, b0.x, b0.y);
 #pragma unroll
-        for (int m = 0; m < 2; m++) few_mma(acc[m][n], w[m][0].x, w[m][2].x, w[m][0].y, w[m][2].y, b0.x, b0.y);
+      for (int m = 0; m < 2; m++) few_mma(acc[m], w[m][0].z, w[m][2].z, w[m][0].w, w[m][2].w, b0.z, b0.w);
 #pragma unroll
-        for (int m = 0; m < 2; m++) few_mma(acc[m][n], w[m][0].z, w[m][2].z, w[m][0].w, w[m][2].w, b0.z, b0.w);
+      for (int m = 0; m < 2; m++) few_mma(acc[m], w[m][1].x, w[m][3].x, w[m][1].y, w[m][3].y, b1.x, b1.y);
 #pragma unroll
-        for (int m = 0; m < 2; m++) few_mma(acc[m][n], w[m][1].x, w[m][3].x, w[m][1].y, w[m][3].y, b1.x, b1.y);
-#pragma unroll
-        for (int m = 0; m < 2; m++) few_mma(acc[m][n], w[m][1].z, w[m][3].z, w[m][1].w, w[m][3].w, b1.z, b1.w);
-      }
+      for (int m = 0; m < 2; m++) few_mma(acc[m], w[m][1].z, w[m][3].z, w[m][1].w, w[m][3].w, b1.z, b1.w);
       __syncwarp();  // every lane's reads of the block have been consumed by the products above
       if (lane == 0 && next < total) issue();
       if (++slot == lay.stages) slot = 0, phase ^= 1;
     }
-    // the warps' shares of the 32 x 8 NT scores, [token][row]
-    float* out = red + (buf * FEW_WARPS + warp) * FEW_ROWS * 8 * NT;
+    // the warps' shares of the 32 x 8 scores, [token][row]
+    float* out = red + (buf * FEW_WARPS + warp) * FEW_ROWS * FEW_TOKENS;
 #pragma unroll
-    for (int n = 0; n < NT; n++)
+    for (int m = 0; m < 2; m++)
 #pragma unroll
-      for (int m = 0; m < 2; m++)
-#pragma unroll
-        for (int j = 0; j < 4; j++) out[(n * 8 + 2 * t + (j & 1)) * FEW_ROWS + m * 16 + g + (j & 2) * 4] = acc[m][n][j];
+      for (int j = 0; j < 4; j++) out[(2 * t + (j & 1)) * FEW_ROWS + m * 16 + g + (j & 2) * 4] = acc[m][j];
     if (__syncthreads_or(!ok)) {  // the same answer in every thread
       ok = false;
       break;
     }
-#pragma unroll
-    for (int o = 0; o < OWN; o++) {
-      const int i = threadIdx.x + o * FEW_WARPS * 32;
-      const int token = i / FEW_ROWS, v = group * FEW_ROWS + i % FEW_ROWS;
-      if (token >= T) continue;
+    if (token < T) {
+      const int v = group * FEW_ROWS + lane;
       float sc = 0.f;
 #pragma unroll
-      for (int w = 0; w < FEW_WARPS; w++) sc += red[(buf * FEW_WARPS + w) * FEW_ROWS * 8 * NT + i];
+      for (int w = 0; w < FEW_WARPS; w++) sc += red[(buf * FEW_WARPS + w) * FEW_ROWS * FEW_TOKENS + threadIdx.x];
       if (GRAD) {
         if (v < width) {
-          float p = v < V ? e_coef[o] * p_ex2(fmaf(sc, P_LOG2E, -e_lz[o])) : 0.f;
-          if (v == e_t[o]) p -= e_g[o];
+          float p = v < V ? e_coef * p_ex2(fmaf(sc, P_LOG2E, -e_lz)) : 0.f;
+          if (v == e_t) p -= e_g;
           d[token * ldd + v] = __float2bfloat16_rn(p);
         }
       } else if (v < V) {
-        if (v == e_t[o]) args.tgt[token] = sc;
-        const float nm = fmaxf(run_m[o], sc);
+        if (v == e_t) args.tgt[token] = sc;
+        const float nm = fmaxf(run_m, sc);
         const float base = nm == -INFINITY ? 0.f : nm * P_LOG2E;
-        run_s[o] = run_s[o] * p_ex2(fmaf(run_m[o], P_LOG2E, -base)) + p_ex2(fmaf(sc, P_LOG2E, -base));
-        run_m[o] = nm;
+        run_s = run_s * p_ex2(fmaf(run_m, P_LOG2E, -base)) + p_ex2(fmaf(sc, P_LOG2E, -base));
+        run_m = nm;
       }
     }
     buf ^= 1;
@@ -293,21 +278,16 @@ ce_few_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant_
     return;
   }
   if (!GRAD) {
+    float m = run_m, s = run_s;
 #pragma unroll
-    for (int o = 0; o < OWN; o++) {
-      // the 32 rows of a token sit in the 32 lanes of a warp
-      float m = run_m[o], s = run_s[o];
-#pragma unroll
-      for (int k = 16; k > 0; k >>= 1) {
-        const float om = __shfl_xor_sync(0xffffffffu, m, k), os = __shfl_xor_sync(0xffffffffu, s, k);
-        const float nm = fmaxf(m, om);
-        const float base = nm == -INFINITY ? 0.f : nm * P_LOG2E;
-        s = s * p_ex2(fmaf(m, P_LOG2E, -base)) + os * p_ex2(fmaf(om, P_LOG2E, -base));
-        m = nm;
-      }
-      const int i = threadIdx.x + o * FEW_WARPS * 32;
-      if (i % FEW_ROWS == 0 && i / FEW_ROWS < T) args.part[static_cast<int64_t>(blockIdx.x) * T + i / FEW_ROWS] = make_float2(m, s);
+    for (int k = 16; k > 0; k >>= 1) {
+      const float om = __shfl_xor_sync(0xffffffffu, m, k), os = __shfl_xor_sync(0xffffffffu, s, k);
+      const float nm = fmaxf(m, om);
+      const float base = nm == -INFINITY ? 0.f : nm * P_LOG2E;
+      s = s * p_ex2(fmaf(m, P_LOG2E, -base)) + os * p_ex2(fmaf(om, P_LOG2E, -base));
+      m = nm;
     }
+    if (lane == 0 && token < T) args.part[static_cast<int64_t>(blockIdx.x) * T + token] = make_float2(m, s);
   }
 }
 
@@ -359,15 +339,15 @@ int ce_band(int M, int K) {
 // 123; level from H = 1024 on.  The plain products' epilogues gain nothing and keep four.
 constexpr int CE_WARPS = 8;
 
-template <bool A_MN, bool B_MN, int OUT, class EXT>
+template <bool A_MN, bool B_MN, int OUT, int ST = 0, class EXT>
 int ce_launch(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& td, int M, int N, int K, const PSched& sched, const CUtensorMap& tws, const EXT& ext,
               int* status, int num_sms, cudaStream_t stream) {
-  constexpr int EW = OUT == P_OUT_CE_STATS || OUT == P_OUT_CE_GRAD ? CE_WARPS : P_EPI_WARPS;
-  constexpr int STAGES = OUT == P_OUT_CE_GRAD ? P_MAX_STAGES - 1 : P_MAX_STAGES;
+  constexpr int EW = p_ce_stats(OUT) || OUT == P_OUT_CE_GRAD ? CE_WARPS : P_EPI_WARPS;
+  constexpr int STAGES = ST ? ST : OUT == P_OUT_CE_GRAD ? P_MAX_STAGES - 1 : P_MAX_STAGES;
   auto kern = gemm2_tcgen05_kernel<A_MN, B_MN, OUT, STAGES, EXT, EW>;
   static bool done[64] = {};
   if (int rc = ce_configure(kern, done, P_SMEM)) return rc;
-  if (OUT == P_OUT_CE_STATS) {  // its warp groups exchange registers: the block has to be launched with as many as they share out
+  if (p_ce_stats(OUT)) {  // its warp groups exchange registers: the block has to be launched with as many as they share out
     static int regs = -1;
     if (regs < 0) {
       cudaFuncAttributes fa;
@@ -379,6 +359,7 @@ int ce_launch(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& t
   static const PPeerMaps no_maps = {};
   int pairs = num_sms / 2;
   if (sched.total_units < pairs) pairs = sched.total_units;
+  if constexpr (OUT == P_OUT_CE_STATS_T) pairs = pairs / ((N + ext.tile_n - 1) / ext.tile_n) * ((N + ext.tile_n - 1) / ext.tile_n);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(2 * pairs), 1, 1);
   cfg.blockDim = dim3(p_threads(OUT, EW), 1, 1);
@@ -392,7 +373,7 @@ int ce_launch(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& t
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // see ce_launch_next
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = OUT == P_OUT_CE_STATS ? 1 : 2;  // the statistics are their entry point's first kernel
+  cfg.numAttrs = p_ce_stats(OUT) ? 1 : 2;  // the statistics are their entry point's first kernel
   if (cudaLaunchKernelEx(&cfg, kern, ta, tb, td, M, N, K, ce_band(M, K), status, PFuse(), no_maps, sched, tws, ta, ext) != cudaSuccess) {
     cudaGetLastError();
     return NTB_ERR_LAUNCH;
@@ -410,18 +391,13 @@ PSched ce_whole_tiles(int M, int N, int K, bool& fits) {
   return sc;
 }
 
-// Groups of 8 tokens of the few-token kernel, 0: the GEMM kernel.  The tokens' padded copy may take up to 128 KB, the rings the rest.
-// Forward pass, us, this kernel | GEMM kernel: 16 x 256 x 128256 30 | 36, 1 x 2048 x 128256 85 | 107, 16 x 4096 x 128256 172 | 206, 1 x 8192 x
-// 128256 323 | 375; with four groups 32 x 1024 x 128256 took 82 against 65, so more than 16 tokens go to the GEMM kernel.
-int ce_few_groups(int T, int H) {
-  if (T > FEW_MAX_TOKENS) return 0;
-  const int nt = (T + 7) / 8;
-  return static_cast<int64_t>(nt) * 8 * H <= 65536 ? nt : 0;
-}
+// Whether the few-token kernel takes the call.  The tokens' padded copy takes shared memory from the rings.  Forward pass, us, this kernel | the turned
+// product (ce_turned_tile): 1 x 256 x 32000 10 | 12, 1 x 2048 x 128256 85 | 89, 8 x 4096 x 128256 161 | 175, 1 x 8192 x 128256 367 | 338.
+bool ce_few(int T, int H) { return T <= FEW_TOKENS && H <= 4096; }
 
 // Rows of a load of the tokens: no more than there are, in steps of the swizzle's 8 rows.  A load fills rows past the end with zeros, but
-// slowly: forward pass, us, loads of 128 rows | of the tokens: 17 x 1024 x 128256 79 | 64, 17 x 2048 x 128256 128 | 108, 33 x 1024 x 128256 70 |
-// 65, level from 64 tokens on.  What is not loaded has to be zero all the same: leftovers in its place took 4 % (power, not work).
+// slowly: gradient of the scores, us, loads of 128 rows | of the tokens: 17 x 1024 x 128256 61 | 56, 17 x 2048 x 128256 109 | 98, level from 64
+// tokens on.  What is not loaded has to be zero all the same: leftovers in its place took 4 % (power, not work).
 int ce_a_rows(int T) { return T < P_BLOCK_M ? (T + 7) / 8 * 8 : P_BLOCK_M; }
 
 bool few_map(CUtensorMap* m, const void* ptr, int64_t rows, int64_t k, int64_t ld, int box_rows) {
@@ -438,27 +414,40 @@ int few_grid(int rows, int num_sms) {
   return groups < num_sms ? groups : num_sms;
 }
 
-template <int NT, bool GRAD>
+template <bool GRAD>
 int few_launch(const void* x, int64_t ldx, const void* w, int64_t ldw, int T, int V, int H, const PCeArgs& a, void* d, int64_t ldd, int width, int* status, int num_sms,
                cudaStream_t stream) {
-  auto kern = ce_few_kernel<NT, GRAD>;
+  auto kern = ce_few_kernel<GRAD>;
   static bool done[64] = {};
   if (int rc = ce_configure(kern, done, FEW_SMEM)) return rc;
   CUtensorMap tx, tw;
-  if (!few_map(&tx, x, T, H, ldx, NT * 8) || !few_map(&tw, w, V, H, ldw, FEW_ROWS)) return NTB_ERR_ARG;
+  if (!few_map(&tx, x, T, H, ldx, FEW_TOKENS) || !few_map(&tw, w, V, H, ldw, FEW_ROWS)) return NTB_ERR_ARG;
   __nv_bfloat16* out = static_cast<__nv_bfloat16*>(d);
   if (GRAD) return ce_launch_next(kern, few_grid(width, num_sms), FEW_WARPS * 32, FEW_SMEM, stream, tx, tw, T, V, H / 64, a, out, ldd, width, status);
   kern<<<few_grid(V, num_sms), FEW_WARPS * 32, FEW_SMEM, stream>>>(tx, tw, T, V, H / 64, a, out, ldd, width, status);
   return ntb_check_launch();
 }
-template <bool GRAD>
-int few_dispatch(int nt, const void* x, int64_t ldx, const void* w, int64_t ldw, int T, int V, int H, const PCeArgs& a, void* d, int64_t ldd, int width, int* status, int num_sms,
-                 cudaStream_t stream) {
-  if (nt == 1) return few_launch<1, GRAD>(x, ldx, w, ldw, T, V, H, a, d, ldd, width, status, num_sms, stream);
-  return few_launch<2, GRAD>(x, ldx, w, ldw, T, V, H, a, d, ldd, width, status, num_sms, stream);
-}
 
 bool ce_operand_ok(const void* p, int64_t ld) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld % 64 == 0; }
+
+// Tokens per tile where the product is turned around (P_OUT_CE_STATS_T: weight rows in the place of A), 0: not turned.  A tile of the product as it
+// stands has 256 tokens, empty rows and all; turned around its width is what there is, in steps of 32.  With up to 128 tokens that leaves the
+// tensor cores half idle and room for two more stages of the weight, and the pass runs at the rate of the memory.  Forward pass, us, as it stands |
+// turned: 32 x 1024 x 128256 66 | 49, 64 x 2048 x 128256 112 | 84 (6.25 TB/s), 128 x 4096 x 128256 211 | 175, 333 x 768 x 50257 39 | 36, 256 x 2048 x
+// 128256 149 | 127, 448 x 2048 x 128256 260 | 211, 1024 x 2048 x 128256 448 | 423, 1024 x 8192 x 128256 1741 | 1686.  The epilogue does more for a
+// score (it is turned back in shared memory), which wide tiles show where the products are short: 256 x 512 x 32000 18 | 20, 768 x 1024 x 128256
+// 168 | 174.  Behind 1024 tokens the two are level at best (1536 x 4096 x 128256 1300 | 1304), and token tiles that do not divide the pairs leave
+// some idle: 4096 x 2048 x 128256 1500 | 1700.
+int ce_turned_tile(int T, int H, int num_sms) {
+  const int tiles = (T + P_BLOCK_N - 1) / P_BLOCK_N;
+  const int tile = ((T + tiles - 1) / tiles + 31) / 32 * 32;
+  return T <= 1024 && tiles <= num_sms / 2 && (tile <= 192 || H >= (T <= P_BLOCK_N ? 1024 : 2048)) ? tile : 0;
+}
+// Pairs of CTAs that share the vocabulary for one of the token tiles.
+int ce_turned_pairs(int T, int V, int tile, int num_sms) {
+  const int token_tiles = (T + tile - 1) / tile, pairs = num_sms / 2 / token_tiles, v_tiles = (V + 2 * P_BLOCK_M - 1) / (2 * P_BLOCK_M);
+  return pairs < v_tiles ? pairs : v_tiles;
+}
 
 int ce_stats(const void* x, int64_t ldx, const void* w, int64_t ldw, const int64_t* target, int64_t vocab_start, int T, int V, int H, void* part, float* tgt, int* status,
              int num_sms, cudaStream_t stream) {
@@ -467,12 +456,24 @@ int ce_stats(const void* x, int64_t ldx, const void* w, int64_t ldw, const int64
   a.col0 = vocab_start;
   a.part = static_cast<float2*>(part);
   a.tgt = tgt;
-  if (const int nt = ce_few_groups(T, H)) return few_dispatch<false>(nt, x, ldx, w, ldw, T, V, H, a, nullptr, 0, 0, status, num_sms, stream);
+  if (ce_few(T, H)) return few_launch<false>(x, ldx, w, ldw, T, V, H, a, nullptr, 0, 0, status, num_sms, stream);
   bool fits;
-  const PSched sched = ce_whole_tiles(T, V, H, fits);
   CUtensorMap ta, tb;
-  a.a_rows = ce_a_rows(T);
-  if (!fits || !p_map_kmajor(&ta, x, T, H, ldx, a.a_rows) || !p_map_kmajor(&tb, w, V, H, ldw)) return NTB_ERR_ARG;
+  if (const int tile = ce_turned_tile(T, H, num_sms)) {
+    const int token_tiles = (T + tile - 1) / tile;
+    PSched sched;
+    sched.total_units = sched.full_units = (V + 2 * P_BLOCK_M - 1) / (2 * P_BLOCK_M) * token_tiles;
+    a.tile_n = tile;
+    if (!p_map_kmajor(&ta, w, V, H, ldw) || !p_map_kmajor(&tb, x, T, H, ldx, tile / 2)) return NTB_ERR_ARG;
+    switch ((tile + 63) / 64) {
+      case 1: return ce_launch<false, false, P_OUT_CE_STATS_T, 8>(ta, tb, ta, V, T, H, sched, ta, PCeTurned<1>{a}, status, num_sms, stream);
+      case 2: return ce_launch<false, false, P_OUT_CE_STATS_T, 8>(ta, tb, ta, V, T, H, sched, ta, PCeTurned<2>{a}, status, num_sms, stream);
+      case 3: return ce_launch<false, false, P_OUT_CE_STATS_T>(ta, tb, ta, V, T, H, sched, ta, PCeTurned<3>{a}, status, num_sms, stream);
+      default: return ce_launch<false, false, P_OUT_CE_STATS_T>(ta, tb, ta, V, T, H, sched, ta, PCeTurned<4>{a}, status, num_sms, stream);
+    }
+  }
+  const PSched sched = ce_whole_tiles(T, V, H, fits);
+  if (!fits || !p_map_kmajor(&ta, x, T, H, ldx) || !p_map_kmajor(&tb, w, V, H, ldw)) return NTB_ERR_ARG;
   return ce_launch<false, false, P_OUT_CE_STATS>(ta, tb, ta, T, V, H, sched, ta, a, status, num_sms, stream);
 }
 
@@ -486,7 +487,7 @@ int ce_dlogits(const void* x, int64_t ldx, const void* w, int64_t ldw, const int
   a.logz = logz;
   a.coef = coef;
   a.g = gn;
-  if (const int nt = ce_few_groups(T, H)) return few_dispatch<true>(nt, x, ldx, w, ldw, T, V, H, a, d, ldd, static_cast<int>(width), status, num_sms, stream);
+  if (ce_few(T, H)) return few_launch<true>(x, ldx, w, ldw, T, V, H, a, d, ldd, static_cast<int>(width), status, num_sms, stream);
   bool fits;
   const PSched sched = ce_whole_tiles(T, V, H, fits);
   CUtensorMap ta, tb, td;
@@ -593,8 +594,9 @@ NTB_EXPORT int ntb_linear_ce_forward(const void* x, int64_t ldx, const void* w, 
   if (T <= 0 || V <= 0 || H <= 0 || H % 64 || !ce_operand_ok(x, ldx) || !ce_operand_ok(w, ldw) || (reinterpret_cast<uintptr_t>(part) & 7) || num_sms < 2 || !out0 || !out1 || (!out2 && (!finish || z_coef > 0.f)) ||
       !p_get_encode())
     return NTB_ERR_ARG;
-  // partial statistics per token: one of every half tile (the last may have no columns: (-inf, 0)), or one of every CTA
-  const int tiles = ce_few_groups(T, H) ? few_grid(V, num_sms) : (V + P_BLOCK_N - 1) / P_BLOCK_N * (CE_WARPS / 4);
+  // partial statistics per token: one of every CTA, or one of every half tile (the last may have no columns: (-inf, 0))
+  const int turned = ce_turned_tile(T, H, num_sms);
+  const int tiles = ce_few(T, H) ? few_grid(V, num_sms) : turned ? 2 * ce_turned_pairs(T, V, turned, num_sms) : (V + P_BLOCK_N - 1) / P_BLOCK_N * (CE_WARPS / 4);
   float* tgt = part + static_cast<int64_t>(tiles) * 2 * T;
   const int rc = ce_stats(x, ldx, w, ldw, target, vocab_start, T, V, H, part, tgt, status, num_sms, stream);
   if (rc != NTB_OK) return rc;

@@ -189,10 +189,12 @@ def check(x, w, y, g, z=0.0, main_grad=None):
 
 
 SHAPES = [(1, 64, 1), (1, 64, 257), (3, 128, 255), (2, 192, 64), (257, 64, 1000), (128, 448, 4096), (130, 4096, 513), (515, 576, 9001), (64, 1024, 20011), (2049, 128, 777), (300, 1088, 1000), (257, 4096, 700), (40, 2112, 3000)]
-# up to 16 tokens that fit beside the rings take their own kernel: its token groups, odd block counts, last rows, and the sizes just past it
+# up to 8 tokens take their own kernel: odd block counts, last rows, and the sizes just past it
 SHAPES += [(1, 2048, 5003), (8, 8192, 300), (9, 4096, 1000), (16, 4160, 129), (17, 64, 16), (31, 576, 2400), (32, 2048, 4111), (33, 64, 100), (7, 64, 40000), (1, 8256, 33)]
 # GEMM kernel with operands of fewer rows than a load takes otherwise
 SHAPES += [(24, 4096, 600), (113, 320, 1500), (121, 1152, 260), (127, 64, 70000), (129, 1088, 300)]
+# the product turned around: its tile widths, several token tiles, fewer vocabulary tiles than CTA pairs, and the sizes past it
+SHAPES += [(60, 64, 1), (65, 2048, 9000), (192, 128, 70000), (200, 64, 70), (255, 1088, 300), (333, 256, 5000), (450, 2048, 129), (520, 192, 3001), (1000, 2112, 1300), (1024, 2048, 257), (1025, 2048, 257)]
 
 
 @gpu
@@ -200,6 +202,26 @@ SHAPES += [(24, 4096, 600), (113, 320, 1500), (121, 1152, 260), (127, 64, 70000)
 @pytest.mark.parametrize("z", [0.0, 1e-2])
 def test_kernels_match_the_definition(T, H, V, z):
     check(*inputs(T, H, V, DEV, torch.bfloat16), z=z)
+
+
+@gpu
+@pytest.mark.parametrize("T", [3, 40, 100, 130, 300, 1100])
+def test_masked_vocabulary_and_tokens_that_are_not_finite(T):
+    """Rows of the weight whose scores are -inf or the lowest numbers take no part; a token that is not finite spoils its own loss alone."""
+    x, w, y, _ = inputs(T, 128, 700, DEV, torch.bfloat16, seed=5)
+    x = x.abs() + 0.25  # positive: a weight row of -inf scores -inf, without 0 * inf
+    w[17], w[600] = float("-inf"), -1e36
+    y[(y == 17) | (y == 600)] = 5
+    bad = [1, T - 1]
+    x[1, 7], x[T - 1, 100] = float("nan"), float("inf")
+    loss = linear_cross_entropy(x, w, y)
+    assert loss[bad].isnan().all()
+    good = [t for t in range(T) if t not in bad]
+    scores = x[good].double() @ w.double().t()
+    want = torch.logsumexp(scores, 1) - scores.gather(1, y[good][:, None])[:, 0]
+    kept = [v for v in range(700) if v not in (17, 600)]
+    ds = (x[good].double() @ w[kept].double().abs().t()).amax(dim=1) * (128 / 16 + 2) * 2.0**-23 + 2.0**-20
+    within(loss[good], want, 2 * ds + 2.0**-20 * want.abs(), "loss")
 
 
 @gpu
