@@ -48,10 +48,20 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(1) == 1 and t.stride(0) >= t.shape[1] and t.stride(0) % 64 == 0 and t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
 
 
+_key = lru_cache(maxsize=None)(str)  # of a device: str(device) takes longer than a launch needs for anything else
+
+
 def _status(device) -> torch.Tensor:
-    if str(device) not in native_gemm._STATUS and torch.cuda.is_current_stream_capturing():
-        raise native.NativeKernelError("the first tensor-core call on a device cannot be captured into a CUDA graph: run it once before the capture")
-    return native_gemm.status_word(device)
+    word = native_gemm._STATUS.get(_key(device))
+    if word is None:
+        if torch.cuda.is_current_stream_capturing():
+            raise native.NativeKernelError("the first tensor-core call on a device cannot be captured into a CUDA graph: run it once before the capture")
+        word = native_gemm.status_word(device)
+    return word
+
+
+def _sms(device) -> int:
+    return native_gemm._SMS.get(_key(device)) or native_gemm._sms(device)
 
 
 def forward(x2: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, vocab_start: int, finish: bool, z_coef: float = 0.0):
@@ -60,7 +70,7 @@ def forward(x2: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, vocab_
     x2, weight = _rows(x2), _rows(weight)
     (T, H), V, dev = x2.shape, weight.shape[0], x2.device
     with native.on_device(dev):
-        status, sms = _status(dev), native_gemm._sms(dev)
+        status, sms = _status(dev), _sms(dev)
         part = torch.empty((max((V + 255) // 256 * 4, 2 * sms) + 1) * T, dtype=torch.float32, device=dev)  # per part two numbers, and the target's score
         a, b = torch.empty(T, dtype=torch.float32, device=dev), torch.empty(T, dtype=torch.float32, device=dev)
         c = torch.empty(T, dtype=torch.float32, device=dev) if z_coef > 0 or not finish else None
@@ -95,7 +105,7 @@ def backward(x2, weight, target, logz, g, gz: Optional[torch.Tensor], z_coef: fl
     ``main_grad`` (fp32 [V, H]) dw is added to it and None is returned in its place."""
     x2, weight = _rows(x2), _rows(weight)
     (T, H), V, dev = x2.shape, weight.shape[0], x2.device
-    sms = native_gemm._sms(dev)
+    sms = _sms(dev)
     width, pitch, split, words, offsets = _backward_plan(T, V, H, sms, need_dx, PIECE_ELEMENTS, PIECE_MIN)
     with native.on_device(dev):
         scratch = torch.empty(words, dtype=torch.float32, device=dev)

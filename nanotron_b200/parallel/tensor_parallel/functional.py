@@ -282,12 +282,17 @@ def sharded_cross_entropy_with_z_loss(sharded_logits, target, group, dtype=None,
 
 
 # ----------------------------------------------------------------------------- cross entropy of a vocabulary-sharded linear head
+def _row(t, dtype):
+    """``t`` as a contiguous vector of ``dtype``; itself where it is one (three calls less: small steps are bound by the host)."""
+    return t if t.dim() == 1 and t.dtype == dtype and t.is_contiguous() else t.reshape(-1).to(dtype).contiguous()
+
+
 def _linear_cross_entropy_forward(x, weight, target, group, z_loss_coef: float):
     tp = group.size() if group is not None else 1
     rank = dist.get_rank(group) if tp > 1 else 0
     lead = x.shape[:-1]
     x2 = x if len(lead) == 1 else x.reshape(-1, x.shape[-1])
-    tgt = target.reshape(-1).to(torch.int64).contiguous()
+    tgt = _row(target, torch.int64)
     vocab_start = rank * weight.shape[0]
     z = None
     if x2.shape[0] == 0:
@@ -333,10 +338,11 @@ class _LinearCrossEntropy(torch.autograd.Function):
         if x2.shape[0] == 0:
             return (x2.new_zeros(ctx.shape) if need_dx else None), (torch.zeros_like(weight) if need_dw else None), None, None, None
         wide = logz.dtype
-        g = grad_loss.reshape(-1).to(wide).contiguous()
-        gz = grad_z.reshape(-1).to(wide).contiguous() if ctx.z > 0 else None
+        g, gz = _row(grad_loss, wide), (_row(grad_z, wide) if ctx.z > 0 else None)
         dx, dw = ops.linear_ce_backward(x2, weight, tgt, logz, g, gz, ctx.z, ctx.vocab_start, need_dx, need_dw)
-        return (dx.view(ctx.shape) if need_dx else None), dw, None, None, None
+        if need_dx and len(ctx.shape) != 2:
+            dx = dx.view(ctx.shape)
+        return dx, dw, None, None, None
 
 
 def _check_linear_cross_entropy(x, weight, target):
