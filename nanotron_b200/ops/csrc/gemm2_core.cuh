@@ -427,7 +427,7 @@ gemm2_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
               ptx::tc_fence_after();
               const uint32_t sa = ptx::smem_u32(smem + s * STAGE);
               const uint32_t sb = sa + P_A_BYTES;
-  #pragma unroll
+#pragma unroll
               for (int k = 0; k < P_BLOCK_K / P_UMMA_K; k++) {
                 const uint64_t adesc = A_MN ? ptx::make_smem_desc(sa + k * P_UMMA_K * 128, P_BLOCK_K * 128, 1024) : ptx::make_smem_desc(sa + k * P_UMMA_K * 2, 16, 1024);
                 const uint64_t bdesc = B_MN ? ptx::make_smem_desc(sb + k * P_UMMA_K * 128, P_BLOCK_K * 128, 1024) : ptx::make_smem_desc(sb + k * P_UMMA_K * 2, 16, 1024);
