@@ -14,7 +14,9 @@ import torch
 
 from nanotron_b200.ops import native, native_gemm
 
-PIECE_ELEMENTS = 1 << 27  # scores of one piece of the backward pass: 256 MiB of bf16
+# Scores of one piece of the backward pass: 512 MiB of bf16.  Backward pass with 128 | 256 | 512 MiB, us: 4096 x 1024 x 151936 3604 | 3230 | 3051,
+# 8192 x 2048 x 128256 11288 | 10143 | 10051, 8192 x 4096 x 128256 20585 | 20487 | 20015 (fewer sums of dx, fuller last rounds of tiles).
+PIECE_ELEMENTS = 1 << 28
 PIECE_MIN = 4096          # narrowest piece: below it the sums of dx over the pieces cost more than the pieces save
 
 
